@@ -166,7 +166,7 @@ def _blocks(x, S, T, H, D):
 
 def _quantise(x):
     """Codes and scales of blocks [..., 32, D]; the quotient in 64 bits, where values next to a border stay on their side."""
-    scale = x.abs().amax((-2, -1)) / 127
+    scale = x.abs().amax((-2, -1)) / torch.full((), 127.0, device="cuda")  # (by a number, torch multiplies with 1 / 127)
     code = (x.double() / scale.double()[..., None, None]).round().clamp(-127, 127)
     return torch.where(scale[..., None, None] > 0, code, torch.zeros_like(code)).to(torch.int8), scale
 
@@ -206,7 +206,8 @@ def _adjusted(s):
     seen.scatter_add_(1, torch.where(ids < 0, V, ids), torch.ones_like(ids, dtype=torch.float32))
     seen = seen[:, :V]
     there = seen > 0
-    x = torch.where(there, torch.where(x > 0, x / RULES["repetition"], x * RULES["repetition"]), x)
+    r = torch.full((), RULES["repetition"], device="cuda")
+    x = torch.where(there, torch.where(x > 0, x / r, x * r), x)
     x = x - seen * RULES["frequency"] - torch.where(there, RULES["presence"], 0.0)
     if s["bias"] is not None:
         x = x + s["bias"]
@@ -438,7 +439,7 @@ def _stored64(x):
     for part, rows in ((x[:full].double().reshape(-1, BLOCK * x.shape[1]), slice(0, full)), (x[full:].double().reshape(-1, (T - full) * x.shape[1]) if T > full else None, slice(full, T))):
         if part is None or not part.numel():
             continue
-        step = (part.abs().max(1).values.float() / 127).double().unsqueeze(1)
+        step = (part.abs().max(1).values / 127).float().double().unsqueeze(1)
         code = torch.where(step > 0, torch.round(part / step.clamp_min(1e-300)), torch.zeros_like(part))
         out[rows] = (code.clamp(-127, 127) * step).reshape(-1, x.shape[1])
     return out
