@@ -6,8 +6,8 @@ the glue ops its encoder/decoder forwards call between them - on top of the C-AB
 library `libfa_cuda.so` (include/fa_cuda.h).  There is no CPU fallback: importing works
 anywhere, creating a context without the built library or without a B200 raises.
 """
-from .context import ACT, CudaContext, CudaError, PackedBytes, StagedRead, Tensor, create_context
+from .context import ACT, CudaContext, CudaError, KvCache8, PackedBytes, StagedRead, Tensor, create_context
 from ._lib import library_path, load_library
 
-__all__ = ["ACT", "CudaContext", "CudaError", "PackedBytes", "StagedRead", "Tensor", "create_context",
+__all__ = ["ACT", "CudaContext", "CudaError", "KvCache8", "PackedBytes", "StagedRead", "Tensor", "create_context",
            "library_path", "load_library"]

@@ -40,6 +40,11 @@ class ConformerLayer(C.Structure):
                          "pw1", "pw2", "qb", "kb", "vb", "qkvb", "outb", "pw1b", "pw2b", "pbu", "pbv", "dw", "dwb")]
 
 
+class LogitRules(C.Structure):
+    _fields_ = [("history", P), ("n", I), ("repetition", C.c_float), ("presence", C.c_float), ("frequency", C.c_float),
+                ("bias", P), ("mask", P), ("mask_rows", P)]
+
+
 # name -> argtypes (every function returns int except fa_last_error)
 SIGNATURES = {
     "fa_ctx_create": [I, PP],
@@ -101,6 +106,12 @@ SIGNATURES = {
     "fa_linear_step": [P, P, P, P, C.c_float, P, P, P, I, I, P, I, P, PP],
     "fa_attn_step": [P, P, P, P, I, I, I, PP],
     "fa_attn_step_append": [P, P, P, P, I, I, I, PP],
+    "fa_kv8_create": [P, I, I, I, I, PP],
+    "fa_kv8_free": [P, P],
+    "fa_kv8_write": [P, P, P, P, I, P, P],
+    "fa_kv8_read": [P, P, I, I, PP, PP],
+    "fa_attn_kv8": [P, P, P, I, I, P, PP],
+    "fa_attn_append_kv8": [P, P, P, I, I, P, P, PP],
     "fa_decoder_step": [P, P, I, P, PP, PP, PP, PP, I, I, I, P, P, P, PP],
     "fa_conformer_block": [P, P, P, P, P, I, I, I, I, I, P, P, PP, PP],
     "fa_attn_fused": [P, P, P, P, P, P, P, I, I, I, PP],
@@ -121,6 +132,8 @@ SIGNATURES = {
     "fa_conv_stem_windows": [P, P, P, P, P, P, P, P, I, I, I, I, PP],
     "fa_conv_dw_pw_windows": [P, P, P, P, P, P, I, I, I, I, PP],
     "fa_argmax_rows": [P, P, I, PP],
+    "fa_adjust_logits": [P, P, I, C.POINTER(LogitRules), PP],
+    "fa_pick_adjusted": [P, P, I, C.POINTER(LogitRules), PP],
     "fa_embed_rows": [P, P, P, P, I, PP],
     "fa_log_mel_windows": [P, P, I, C.c_double, I, PP],
     "fa_tdt_create": [P] + [P] * 13 + [PP],

@@ -46,6 +46,18 @@ class PackedBytes:
         self.h, self.nbytes = h, nbytes
 
 
+class KvCache8:
+    """Key and value cache in 8 bits: S streams of `positions` positions, H heads of HD."""
+
+    __slots__ = ("h", "S", "positions", "H", "HD")
+
+    def __init__(self, h: int, S: int, positions: int, H: int, HD: int):
+        self.h, self.S, self.positions, self.H, self.HD = h, S, positions, H, HD
+
+    def __repr__(self):
+        return f"KvCache8({self.S}x{self.positions}, {self.H} heads of {self.HD})"
+
+
 class StagedRead:
     """Single-use staged readback (compute.d.ts:39-45)."""
 
@@ -422,6 +434,41 @@ class CudaContext:
         self._check(self._lib.fa_attn_step_append(self._h, qkv.h, cacheK.h, cacheV.h, n, NH, HD, C.byref(out)))
         return self._wrap(out) if out.value else None
 
+    # -- key and value cache in 8 bits (optional members) ---------------------------------------------
+    def kvCache8(self, S: int, positions: int, H: int, HD: int) -> KvCache8:
+        """An empty cache of S streams: keys and values as 8-bit codes with a scale for each block of 32 positions and head
+        (see fa_kv8_create).  It belongs to no arena: freeKvCache8 gives it back."""
+        out = C.c_void_p()
+        self._check(self._lib.fa_kv8_create(self._h, S, positions, H, HD, C.byref(out)))
+        return KvCache8(out.value, S, positions, H, HD)
+
+    def freeKvCache8(self, cache: KvCache8) -> None:
+        if cache is not None and cache.h:
+            self._check(self._lib.fa_kv8_free(self._h, cache.h))
+            cache.h = None
+
+    def kvWrite8(self, cache: KvCache8, k, v, n: int = 0, *, pos=None, counts=None) -> KvCache8:
+        """k, v [S*T, H*HD] (f32 or f16 storage) into positions n..n+T-1; `pos` [S] gives each stream a start of its own,
+        `counts` [S] how many of its T rows are there."""
+        self._check(self._lib.fa_kv8_write(self._h, cache.h, k.h, v.h, n, self._h_of(pos), self._h_of(counts)))
+        return cache
+
+    def kvRead8(self, cache: KvCache8, row0: int, rows: int):
+        """Positions row0..row0+rows-1 as the values that are stored: (k, v) [S*rows, H*HD]."""
+        k, v = C.c_void_p(), C.c_void_p()
+        self._check(self._lib.fa_kv8_read(self._h, cache.h, row0, rows, C.byref(k), C.byref(v)))
+        return self._wrap(k), self._wrap(v)
+
+    def attnKv8(self, q, cache: KvCache8, HQ: int, n: int, *, lens=None) -> Tensor:
+        """softmax(q K^T) V over the cache's first n positions (or lens [S] of them) for T queries per stream, q [S*T, HQ*HD];
+        HQ / H neighbouring query heads share a key head.  A stream of length 0 gives zeros."""
+        return self._op(self._lib.fa_attn_kv8, q.h, cache.h, HQ, n, self._h_of(lens))
+
+    def attnAppendKv8(self, qkv, cache: KvCache8, HQ: int, n: int = 0, *, pos=None, counts=None) -> Tensor:
+        """The self-attention form: qkv [S*T, (HQ+2H)*HD] = q | k | v of T new tokens per stream; k and v go to positions
+        n..n+T-1 (pos, counts as in kvWrite8), query i attends over positions 0..n+i.  Rows from counts[s] on give zeros."""
+        return self._op(self._lib.fa_attn_append_kv8, qkv.h, cache.h, HQ, n, self._h_of(pos), self._h_of(counts))
+
     # -- layer loops in native code (optional members) -----------------------------------------------
     @staticmethod
     def _live(t) -> Optional[int]:
@@ -549,6 +596,23 @@ class CudaContext:
         """[rows, 2] = {argmax index, max value} per row over the first `ncols` columns (0 = all); the
         host token pick moved to the device."""
         return self._op(self._lib.fa_argmax_rows, x.h, ncols)
+
+    def _rules(self, history, n, repetition, presence, frequency, bias, mask, maskRows):
+        return C.byref(_lib.LogitRules(self._h_of(history), n, repetition, presence, frequency, self._h_of(bias), self._h_of(mask),
+                                       self._h_of(maskRows)))
+
+    def adjustLogits(self, x, ncols: int = 0, *, history=None, n: int = 0, repetition: float = 1.0, presence: float = 0.0,
+                     frequency: float = 0.0, bias=None, mask: Optional[PackedBytes] = None, maskRows=None) -> Tensor:
+        """Optional member: penalties for the tokens of the first n rows of `history` [>=n, rows], a bias [1 or rows, ncols] and a
+        mask of allowed tokens (rows of ceil(ncols/32) little-endian 32-bit words; maskRows [rows] says which row each goes by)
+        -> [rows, ncols] logits, -inf where a token is not allowed (see fa_logit_rules)."""
+        return self._op(self._lib.fa_adjust_logits, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
+
+    def pickAdjusted(self, x, ncols: int = 0, *, history=None, n: int = 0, repetition: float = 1.0, presence: float = 0.0,
+                     frequency: float = 0.0, bias=None, mask: Optional[PackedBytes] = None, maskRows=None) -> Tensor:
+        """Optional member: argmaxRowsIndex of adjustLogits in one pass: [rows, 2] = {index, value}, {-1, -inf} for a row in which
+        no token is allowed."""
+        return self._op(self._lib.fa_pick_adjusted, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
 
     def unshardCols(self, gathered: Tensor, world: int) -> Tensor:
         """[world*M, Ns] column shards stacked along rows -> the row-major [M, world*Ns] product."""

@@ -103,6 +103,7 @@ extern "C" int fa_ctx_destroy(fa_ctx *ctx) {
   }
   for (fa_tensor *t : ctx->tensors) delete t;
   for (fa_bytes *b : ctx->byte_handles) delete b;
+  for (fa_kv8 *c : ctx->kv8s) delete c;
   for (auto &kv : ctx->blocks) cudaFree(kv.first);
   cudaFree(ctx->dev_status);
   cudaFree(ctx->gemv_tickets);
@@ -247,6 +248,9 @@ extern "C" int fa_sync(fa_ctx *ctx) {
   }
   if (st[3] != 0) {
     cudaMemsetAsync(ctx->dev_status, 0, sizeof st, ctx->stream);
+    if (st[3] & kStatusKv8Length)
+      return fa_fail(ctx, FA_ERR_INVALID, "8-bit cache: a stream's length, position or count was outside the cache or the call's rows");
+    if (st[3] & kStatusMaskRow) return fa_fail(ctx, FA_ERR_INVALID, "adjustLogits: a mask row was outside the mask table");
     return fa_fail(ctx, FA_ERR_INVALID, "embedRows: a token id was outside the embedding table");
   }
   return FA_OK;

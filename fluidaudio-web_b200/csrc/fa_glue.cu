@@ -1222,7 +1222,7 @@ __global__ void __launch_bounds__(256) k_embed_rows(const float *__restrict__ ta
   const int s = blockIdx.x;
   int t = (int)idx[(size_t)s * stride];
   if (t < 0 || t >= V) {
-    if (threadIdx.x == 0) atomicOr(status + 3, 1);
+    if (threadIdx.x == 0) atomicOr(status + 3, kStatusTokenId);
     t = 0;
   }
   const float *row = table + (size_t)t * D, *pr = pos + (size_t)n * D;

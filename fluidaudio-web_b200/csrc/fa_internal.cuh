@@ -84,6 +84,15 @@ struct fa_bytes {
   const void *side_scales = nullptr, *side_zp = nullptr;
 };
 
+// Key and value cache of S streams and H heads in 8 bits (fa_kv8.cuh has the layout).
+struct fa_kv8 {
+  int S = 0, P = 0, H = 0, HD = 0;  // streams, positions, heads, head width
+  int HDP = 0, nblk = 0;            // width as stored (a form the attention kernels are built for), blocks of a head
+  uint8_t *codes = nullptr;         // [S][H][nblk] blocks
+  float *tail = nullptr;            // [S][H][2][32][HD]: f32 rows of the block that was written last, keys then values
+  int *tag = nullptr;               // [S][H][2]: which block that is
+};
+
 struct fa_staged {
   float *host = nullptr;     // page-locked snapshot target (f32)
   void *dev_tmp = nullptr;   // device f32 temp when the source is f16 storage
@@ -146,6 +155,7 @@ struct fa_ctx {
   std::unordered_map<int, std::vector<fa_tensor *>> arena_members;
   std::unordered_set<fa_tensor *> tensors;     // every live handle
   std::unordered_set<fa_bytes *> byte_handles;
+  std::unordered_set<fa_kv8 *> kv8s;
   std::unordered_set<fa_staged *> staged;
   // Page-locked staging buffers handed back by consumed reads, for the next stageDownload: allocating and freeing
   // page-locked memory costs milliseconds and synchronises the device, which a read-back per step cannot afford.
@@ -157,7 +167,7 @@ struct fa_ctx {
   // log-mel front end: device tables (filterbank, window, twiddles) per mel count, built on first use
   std::unordered_map<int, void *> mel_tables;
   std::unordered_map<int, int> mel_spans;  // widest filter of each mel count's filterbank, in bins
-  // device-side status word written by kernels whose bounded waits ran out
+  // device-side status words: 0..2 from kernels whose bounded waits ran out, 3 a set of kStatus* bits
   int *dev_status = nullptr;
   int *gemv_tickets = nullptr;  // zeroed arrival counters of the decoder attention's key splits (self-resetting)
   int gemv_ticket_count = 0;
@@ -166,6 +176,9 @@ struct fa_ctx {
   std::unordered_map<void *, fa_graph *> block_owner;
   std::unordered_set<fa_graph *> graphs;
 };
+
+// bits of status word 3: values of index tensors that only the device sees
+enum { kStatusTokenId = 1, kStatusKv8Length = 2, kStatusMaskRow = 4 };
 
 // ---- errors ----------------------------------------------------------------
 

@@ -32,6 +32,7 @@ extern "C" {
 typedef struct fa_ctx fa_ctx;       /* one ComputeContext (compute.d.ts:106) */
 typedef struct fa_tensor fa_tensor; /* Tensor {rows, cols}, storage opaque (compute.d.ts:12-15) */
 typedef struct fa_bytes fa_bytes;   /* PackedBytes from uploadBytes (compute.d.ts:34) */
+typedef struct fa_kv8 fa_kv8;       /* key and value cache in 8 bits */
 typedef struct fa_staged fa_staged; /* StagedRead, single use (compute.d.ts:39-45) */
 typedef struct fa_graph fa_graph;   /* a recorded batch that can be submitted repeatedly */
 
@@ -272,6 +273,30 @@ int fa_linear_step(fa_ctx *ctx, const fa_tensor *x, const fa_tensor *gamma, cons
 int fa_attn_step(fa_ctx *ctx, const fa_tensor *q, const fa_tensor *k, const fa_tensor *v, int H, int HD, int W, fa_tensor **out);
 int fa_attn_step_append(fa_ctx *ctx, const fa_tensor *qkv, fa_tensor *cache_k, fa_tensor *cache_v, int n, int NH, int HD,
                         fa_tensor **out);
+/* ---- key and value cache in 8 bits (optional members; the reference caches f32, raw-whisper-decoder.js:76-100) ----
+ * A cache of S streams x `positions` x H heads of HD.  Keys and values are stored as round(x / scale) in -127..127 with
+ * scale = max|x| / 127 over a block of 32 positions of one head (a block with an infinity or a NaN reads as NaN, one of
+ * zeros as zeros).  A block that is not full is coded from its f32 rows again whenever a row joins it, so what is stored
+ * depends on the rows alone; a call that goes back to a block before the last one written takes that block's earlier rows at
+ * their stored values.  Positions that nothing was written to read as zeros.
+ * `pos`, `counts`, `lens`: optional f32 tensors of one whole number per stream that only the device reads; a value outside the
+ * cache or the call's rows is clamped and makes the next fa_sync fail with FA_ERR_INVALID. */
+int fa_kv8_create(fa_ctx *ctx, int S, int positions, int H, int HD, fa_kv8 **out);
+int fa_kv8_free(fa_ctx *ctx, fa_kv8 *cache);
+/* k, v [S*T, H*HD] (f32 or f16 storage): row i of stream s goes to position n + i, or pos[s] + i; rows i >= counts[s] are
+ * left out. */
+int fa_kv8_write(fa_ctx *ctx, fa_kv8 *cache, const fa_tensor *k, const fa_tensor *v, int n, const fa_tensor *pos,
+                 const fa_tensor *counts);
+/* Positions row0 .. row0 + rows - 1 as the values they stand for: k, v [S*rows, H*HD]. */
+int fa_kv8_read(fa_ctx *ctx, fa_kv8 *cache, int row0, int rows, fa_tensor **out_k, fa_tensor **out_v);
+/* softmax(q K^T) V over positions 0..n-1, or 0..lens[s]-1 (lens[s] <= n), for T queries per stream: q [S*T, HQ*HD] ->
+ * [S*T, HQ*HD].  HQ is a multiple of H: HQ / H neighbouring query heads share a key head.  A stream of length 0 gives zeros.
+ * q carries 1/sqrt(HD) as for fa_attn_step.  f32-grade: operands in 22 bits, sums in f32. */
+int fa_attn_kv8(fa_ctx *ctx, const fa_tensor *q, fa_kv8 *cache, int HQ, int n, const fa_tensor *lens, fa_tensor **out);
+/* The self-attention form: qkv [S*T, (HQ + 2H)*HD] holds q | k | v of T new tokens per stream; writes them as fa_kv8_write
+ * does, then query i attends over positions 0 .. n + i (pos[s] + i) as they are stored now.  Rows i >= counts[s] give zeros. */
+int fa_attn_append_kv8(fa_ctx *ctx, const fa_tensor *qkv, fa_kv8 *cache, int HQ, int n, const fa_tensor *pos,
+                       const fa_tensor *counts, fa_tensor **out);
 /* ---- layer loops of the two transformer engines (optional members) --------------------------------
  * The members above in the engines' order, issued from native code: one call per decoder token or encoder block.  Results
  * belong to the caller's newest arena, everything in between is released. */
@@ -355,6 +380,24 @@ int fa_conv_dw_pw_windows(fa_ctx *ctx, const fa_tensor *x, const fa_tensor *w1, 
  * columns of each row take part (ncols <= 0: all of them) - the tied vocabulary projection is padded
  * with zero columns that must never win (raw-whisper-decoder.js:62-66). */
 int fa_argmax_rows(fa_ctx *ctx, const fa_tensor *x, int ncols, fa_tensor **out);
+/* Rules on logits before a token is picked (optional members; the reference's loop has none of its own, index.ts:80-97).
+ * For column j < ncols (<= 0: all) of a row, c = how often j occurs in the row's history:
+ *   x = c > 0 ? (x > 0 ? x / repetition : x * repetition) : x;  x = x - frequency * c - (c > 0 ? presence : 0);  x = x + bias[j];
+ *   x = allowed ? x : -inf, each step rounded to f32. */
+typedef struct fa_logit_rules {
+  const fa_tensor *history;   /* [>= n, rows of logits] token ids as floats, time-major; ids outside the columns are no token; or NULL */
+  int n;                      /* history rows that count */
+  float repetition, presence, frequency; /* 1, 0, 0: no penalty */
+  const fa_tensor *bias;      /* [1 or rows, >= ncols], or NULL */
+  const fa_bytes *mask;       /* rows of ceil(ncols/32) 32-bit words, bit j%32 of word j/32 set: j is allowed; or NULL */
+  const fa_tensor *mask_rows; /* [rows] which mask row each row of logits goes by (NULL: the one row, or its own); a value
+                                 outside the mask reads row 0 and makes the next fa_sync fail with FA_ERR_INVALID */
+} fa_logit_rules;
+/* -> [rows, ncols] */
+int fa_adjust_logits(fa_ctx *ctx, const fa_tensor *x, int ncols, const fa_logit_rules *rules, fa_tensor **out);
+/* -> [rows, 2] = {index, value} of the first largest allowed value as fa_argmax_rows gives it; {-1, -inf} for a row in which
+ * nothing is allowed or all that is allowed is NaN. */
+int fa_pick_adjusted(fa_ctx *ctx, const fa_tensor *x, int ncols, const fa_logit_rules *rules, fa_tensor **out);
 /* N-sharded products (one process per GPU, each holding a block of output columns): `gathered`
  * [world*M, Ns] is what an all-gather of the ranks' [M, Ns] results leaves; out [M, world*Ns] is the
  * row-major product, out[m, r*Ns + j] = gathered[r*M + m, j].  Ns must be a multiple of 4.  The
