@@ -3,11 +3,10 @@
 // Rows: the G = HQ / H query heads that share a key head times the T queries of a stream, row r = query r / G, head r % G.
 //
 // Arithmetic.  Codes are whole numbers of 8 bits, so they are exact in f16; the other side of each product is split into an
-// f16 value and its f16 residue (22 bits and more), the two sitting in the upper and lower 8 rows of ONE m16n8k16 product, so
-// that a warp's product serves 8 rows with f32-grade operands and f32 sums.  A query row is scaled by a power of two to
-// [1, 2) before the split and the block's scale multiplies the sums afterwards.  Weights are exp(s - the block's own row
-// maximum), so that the largest is 1 whatever the other blocks hold; what the block then adds to the running result is scaled
-// by exp(block maximum - running maximum) times the values' scale, in f32.
+// f16 value and its f16 residue (22 bits and more) and both go through the same product, so that operands are f32-grade and
+// sums are f32.  A query row is scaled by a power of two to [1, 2) before the split and the block's scale multiplies the sums
+// afterwards.  Weights are exp(s - the block's own row maximum), so that the largest is 1 whatever the other blocks hold; what
+// the block then adds to the running result is scaled by exp(block maximum - running maximum) times the values' scale, in f32.
 #include "fa_kv8.cuh"
 #include "fa_tc_common.cuh"
 
@@ -17,6 +16,7 @@ using kv8::kBlock;
 using tc::smem_u32;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
   const float *q;  // query row i of stream s, head h: q + (s*T + i)*ldq + h*HD
@@ -25,23 +25,42 @@ struct AttnParams {
   const float *lens;  // [S] on the device, or NULL: n for all (complete caches)
   kv8::Rows rows;     // causal: where the queries stand
   int causal, n;
-  int H, G, T, HD, nblk, vec;
-  int rowgroups, splits, kper;  // row groups of a unit, its splits and their blocks
-  float *out;                   // [S*T][H*G*HD]
-  __half *y16;                  // packed f16 row operand of out (value plane, then residue plane), or NULL
+  int S, H, G, T, HD, nblk, vec;
+  int rg0, rowgroups; // groups of ROWS rows that this launch takes
+  float *out;         // [S*T][H*G*HD]
+  __half *y16;        // packed f16 row operand of out (value plane, then residue plane), or NULL
   long long lo_off;
-  int R;                        // rows of out
-  float *pacc, *pml;            // splits > 1: [unit][rowgroup][split][8*RG][HDP] and [..][8*RG][2]
-  int *tickets;
+  int R;              // rows of out
+  float *pacc, *pml;  // parts of units that several thread blocks share: [grid][2][rows][HDP] and [..][rows][2]
+  int *tickets;       // [S*H*rowgroups], zero between launches
   int *status;
   unsigned wait_limit;
 };
 
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// What the queries of stream s see: `len` positions at the most, query i limit(i) of them.
+struct Sight {
+  int start, count, len, causal;
+  __device__ __forceinline__ void of(const AttnParams &p, int s, bool &bad) {
+    causal = p.causal, bad = false, start = 0, count = p.T, len = p.n;
+    if (causal) {
+      p.rows.of(s, start, count, bad);
+      len = count > 0 ? start + count : 0;
+    } else if (p.lens) {
+      const float f = p.lens[s];
+      bad = !(f >= 0.0f && f <= (float)p.n);
+      len = f >= 0.0f ? (int)fminf(f, (float)p.n) : 0;
+    }
+  }
+  __device__ __forceinline__ int limit(int i) const { return !causal ? len : i < count ? start + i + 1 : 0; }
+  // a stream of length 0 still has a block that nothing is seen of, so that somebody writes its zeros
+  __device__ __forceinline__ int blocks() const { return max(1, (len + kBlock - 1) / kBlock); }
+};
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t h2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -54,121 +73,235 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
   hi = *(const uint32_t *)&h;
   lo = h2(a - f.x, b - f.y);
 }
-// Four codes u to two pairs of f16 u - 128: 0x6400 | u is 1024 + u.
+// A word of four codes as two pairs of f16 subnormals, code * 2^-24 (see fa_kv8.cuh).
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &b0, uint32_t &b1) {
-  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
-  const __half2 p = __hsub2(*(const __half2 *)&x, bias), q = __hsub2(*(const __half2 *)&y, bias);
-  b0 = *(const uint32_t *)&p, b1 = *(const uint32_t *)&q;
+  b0 = w & 0x807F807Fu, b1 = __byte_perm(w, 0u, 0x2301) & 0x807F807Fu;
 }
-// exp(m - M) for M >= m, 1 where the two are the same infinity
-__device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.0f : __expf(m - M); }
+// two f32 at once
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^(m - M) for M >= m, 1 where the two are the same infinity
+__device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.0f : ex2(m - M); }
 
+// Weights and query rows are scaled by 2^kUp before they are split (f16 ends at 2^16), codes are 2^-24 times themselves.
+constexpr int kUp = 14;
+constexpr float kScoreUnit = 1024.0f * kLog2e;  // 2^(24 - kUp), scores in units of log 2
+constexpr float kValueUnit = 16777216.0f;       // 2^24; the weights' 2^kUp is in their sum too
+
+// Channels 16k + 4t ..+3 of query row `row` for all k, scaled by the power of two that brings its largest element to
+// [2^kUp, 2^(kUp+1)); returns 2^kUp over that scale, NaN for a row that is not finite.  The four lanes of a quad hold the row.
+template <int KS>
+__device__ __forceinline__ float load_row(const AttnParams &p, int s, int h, int row, int t, float (&x)[KS][4]) {
+  const int rr = min(row, p.G * p.T - 1), i = rr / p.G;
+  const float *qp = p.q + ((long long)s * p.T + i) * p.ldq + (h * p.G + rr - i * p.G) * p.HD;
+  uint32_t a = 0;  // largest magnitude, as bits: infinities and NaNs are above all others
+#pragma unroll
+  for (int k = 0; k < KS; k++) {
+    const int d = 16 * k + 4 * t;
+    if (p.vec) {
+      const float4 v = d < p.HD ? *(const float4 *)(qp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[k][e] = d + e < p.HD ? qp[d + e] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < KS; k++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) a = max(a, __float_as_uint(x[k][e]) & 0x7fffffffu);
+  a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
+  a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
+  const int bits = (int)(a >> 23), ex = min(max(bits, kUp + 1), 254);
+  const float f = __int_as_float((254 + kUp - ex) << 23);
+#pragma unroll
+  for (int k = 0; k < KS; k++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[k][e] *= f;
+  return bits < 255 ? __int_as_float(ex << 23) : __int_as_float(0x7fc00000);
+}
+
+// Up to four rows: codes are the ROW operand of the products, 16 positions (or channels) by 16, and the query rows their 8
+// columns, 2r the value and 2r + 1 the residue of row r, so that column sums 2t and 2t + 1 meet in one lane: lane (g, t) has
+// the scores of row t at the four positions 8 (g/2) + 2j + g%2, and channels 16c + g and 16c + 8 + g of row t's result.
 template <int HDP>
-__host__ __device__ constexpr int stages() { return HDP <= 32 ? 6 : HDP <= 64 ? 4 : HDP <= 128 ? 3 : 2; }
+struct FewRows {
+  static constexpr int ROWS = 4, KS = HDP / 16, PITCH = HDP + 8, RESIDENT = 3;
+  uint32_t qb[KS][2];
+  float qs, m, l;
+  uint64_t o[HDP / 8];  // what the weights' values and their residues gave
+  int lim;
 
-// One warp per block of 32 positions; a thread block = one (stream, head), one group of 8*RG rows, one split of the blocks,
-// which its four warps take in turn, each through a ring of its own that the copy engine fills.
-template <int HDP, int RG>
-__global__ void __launch_bounds__(kThreads) k_attn_kv8(const AttnParams p) {
-  constexpr int KS = HDP / 16, NT = HDP / 8, BB = (int)kv8::block_bytes(HDP), NST = stages<HDP>(), ROWS = 8 * RG;
-  extern __shared__ __align__(128) uint8_t ring[];  // [kWarps][NST][BB]; the warps' results afterwards
-  __shared__ __align__(8) uint64_t full[kWarps][NST];
-  __shared__ float sml[kWarps][ROWS][2];
-  __shared__ int last;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint32_t blk = blockIdx.x;
-  const int split = blk % p.splits;
-  blk /= p.splits;
-  const int rg = blk % p.rowgroups, unit = blk / p.rowgroups, s = unit / p.H, h = unit - s * p.H;
-  const int nrows = p.G * p.T;
-  if (threadIdx.x < kWarps * NST) tc::mbar_init(smem_u32(&full[0][0] + threadIdx.x), 1);
-  tc::fence_barrier_init();
-  __syncthreads();
-  fa_grid_dep_sync();
-
-  // how far this group's rows see
-  int start = 0, count = p.T, len = p.n;
-  bool bad = false;
-  if (p.causal) p.rows.of(s, start, count, bad);
-  else if (p.lens) {
-    const float f = p.lens[s];
-    bad = !(f >= 0.0f && f <= (float)p.n);
-    len = f >= 0.0f ? (int)fminf(f, (float)p.n) : 0;
-  }
-  if (bad && threadIdx.x == 0) atomicOr(p.status + 3, kStatusKv8Length);
-  auto limit = [&](int row) {
-    if (row >= nrows) return 0;
-    const int i = row / p.G;
-    return !p.causal ? len : i < count ? start + i + 1 : 0;
-  };
-  const int top_row = min(nrows, (rg + 1) * ROWS) - 1;
-  const int most = p.causal ? (min(top_row / p.G, count - 1) >= rg * ROWS / p.G ? start + min(top_row / p.G, count - 1) + 1 : 0) : len;
-  const int nb = (most + kBlock - 1) / kBlock, b0 = split * p.kper + warp, b1 = min(nb, (split + 1) * p.kper);
-
-  // ring: this warp's blocks b0, b0 + 4, ...
-  const uint8_t *src = p.codes + (size_t)unit * p.nblk * BB;
-  const uint32_t mine = smem_u32(ring) + warp * (NST * BB), bars = smem_u32(&full[warp][0]);
-  auto fetch = [&](int b, int st) {
-    tc::mbar_expect_tx(bars + 8 * st, BB);
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(mine + st * BB),
-                 "l"(src + (size_t)b * BB), "r"(BB), "r"(bars + 8 * st)
-                 : "memory");
-  };
-  if (lane == 0)
-    for (int k = 0; k < NST; k++)
-      if (b0 + k * kWarps < b1) fetch(b0 + k * kWarps, k);
-
-  // query rows as f16 value and residue, scaled to [1, 2)
-  uint32_t qf[RG][KS][4];
-  float qs[RG], m[RG], l[RG], o[RG][NT][2];
-  int lim[RG];
-#pragma unroll
-  for (int r = 0; r < RG; r++) {
-    const int row = rg * ROWS + r * 8 + g;
-    lim[r] = limit(row);
-    m[r] = -INFINITY, l[r] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NT; i++) o[r][i][0] = o[r][i][1] = 0.0f;
-    const int rr = min(row, nrows - 1), i = rr / p.G;
-    const float *qp = p.q + ((long long)s * p.T + i) * p.ldq + (h * p.G + rr - i * p.G) * p.HD;
-    float x[KS][4], a = 0.0f;
-    bool nan = false;
+  __device__ __forceinline__ void start(const AttnParams &p, int s, int h, int row0, const Sight &sight, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float x[KS][4];
+    const float f = load_row<KS>(p, s, h, row0 + (g >> 1), t, x);
+    qs = __shfl_sync(0xffffffffu, f, 8 * t);
 #pragma unroll
     for (int k = 0; k < KS; k++) {
-      const int d = 16 * k + 4 * t;
-      if (p.vec) {
-        const float4 v = d < p.HD ? *(const float4 *)(qp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[k][0] = v.x, x[k][1] = v.y, x[k][2] = v.z, x[k][3] = v.w;
-      } else {
+      uint32_t hi, lo;
+      split2(x[k][0], x[k][1], hi, lo);
+      qb[k][0] = g & 1 ? lo : hi;
+      split2(x[k][2], x[k][3], hi, lo);
+      qb[k][1] = g & 1 ? lo : hi;
+    }
+    lim = row0 + t < p.G * p.T ? sight.limit((row0 + t) / p.G) : sight.len;  // (a row that is not there hinders nobody)
+    m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[k][e] = d + e < p.HD ? qp[d + e] : 0.0f;
+    for (int i = 0; i < HDP / 8; i++) o[i] = 0;
+  }
+
+  // `all`: every row sees every position of the block
+  __device__ __forceinline__ void block(const uint8_t *sb, int first, bool all, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float sc[2][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++) sc[mt][0] = sc[mt][1] = sc[mt][2] = sc[mt][3] = 0.0f;
+    uint32_t w[4 * KS];
+#pragma unroll
+    for (int c = 0; c < KS; c++) {
+      const uint4 w4 = *(const uint4 *)(sb + c * 512 + lane * 16);
+      w[4 * c] = w4.x, w[4 * c + 1] = w4.y, w[4 * c + 2] = w4.z, w[4 * c + 3] = w4.w;
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        uint32_t a0, a1, a2, a3;
+        widen(w[2 * mt * KS + ks], a0, a2);
+        widen(w[(2 * mt + 1) * KS + ks], a1, a3);
+        mma(sc[mt], a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
       }
+    const float2 scales = *(const float2 *)(sb + 2 * kBlock * HDP);
+    const float f = scales.x * kScoreUnit * qs;
+    float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) a = fmaxf(a, fabsf(x[k][e])), nan |= x[k][e] != x[k][e];
+    for (int j = 0; j < 4; j++) v[j] = (sc[j >> 1][2 * (j & 1)] + sc[j >> 1][2 * (j & 1) + 1]) * f;
+    const int n = lim - first - 8 * (g >> 1) - (g & 1);  // position j of this lane is seen if 2j < n
+    if (!all) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = 2 * j < n ? v[j] : -INFINITY;
     }
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const uint32_t quad = 15u << (lane & 28);
-    nan = (__ballot_sync(0xffffffffu, nan) & quad) != 0;
-    int ex = __float_as_int(a) >> 23;  // a >= 0
-    const bool finite = ex < 255 && !nan;
-    ex = min(max(ex, 1), 253);
-    qs[r] = finite ? __int_as_float(ex << 23) * 1.0f : __int_as_float(0x7fc00000);  // 2^(ex - 127); NaN scores for a row that is not finite
-    const float f = finite ? __int_as_float((254 - ex) << 23) : 0.0f;
+    float top = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float ref = top == -INFINITY ? 0.0f : top - kUp, M = fmaxf(m, top), old = rescale(m, M), c = rescale(top, M);
 #pragma unroll
-    for (int k = 0; k < KS; k++) {
-      if (!finite) x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.0f;
-      split2(x[k][0] * f, x[k][1] * f, qf[r][k][0], qf[r][k][1]);
-      split2(x[k][2] * f, x[k][3] * f, qf[r][k][2], qf[r][k][3]);
+    for (int j = 0; j < 4; j++) v[j] = ex2(v[j] - ref);
+    l = fmaf(l, old, ((v[0] + v[1]) + (v[2] + v[3])) * c);
+    m = M;
+    const float add = lim > first ? c * scales.y : 0.0f;  // (a block that a row sees nothing of may hold NaN)
+    const uint64_t add_2 = pair(add, add);
+    if (__any_sync(0xffffffffu, old != 1.0f)) {
+      const uint64_t old_2 = pair(old, old);
+#pragma unroll
+      for (int i = 0; i < HDP / 8; i++) o[i] = mul2(o[i], old_2);
+    }
+    // weights to the lanes that need them as column operand: column g is row g/2's value (g even) or residue, positions 8t..8t+7
+    uint32_t hi[2], lo[2], b[2][2];
+    split2(v[0], v[1], hi[0], lo[0]);
+    split2(v[2], v[3], hi[1], lo[1]);
+    const int even = 8 * t + (g >> 1);
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) {
+      const uint32_t h0 = __shfl_sync(0xffffffffu, hi[kk], even), h1 = __shfl_sync(0xffffffffu, hi[kk], even + 4);
+      const uint32_t l0 = __shfl_sync(0xffffffffu, lo[kk], even), l1 = __shfl_sync(0xffffffffu, lo[kk], even + 4);
+      const uint32_t x = g & 1 ? l0 : h0, y = g & 1 ? l1 : h1;
+      b[kk][0] = __byte_perm(x, y, 0x5410), b[kk][1] = __byte_perm(x, y, 0x7632);
+    }
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      const uint4 w4 = *(const uint4 *)(sb + kBlock * HDP + i * 512 + lane * 16);
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t a0, a1, a2, a3;
+      widen(w4.x, a0, a2);
+      widen(w4.z, a1, a3);
+      mma(acc, a0, a1, a2, a3, b[0][0], b[0][1]);
+      widen(w4.y, a0, a2);
+      widen(w4.w, a1, a3);
+      mma(acc, a0, a1, a2, a3, b[1][0], b[1][1]);
+      o[2 * i] = fma2(pair(acc[0], acc[1]), add_2, o[2 * i]);
+      o[2 * i + 1] = fma2(pair(acc[2], acc[3]), add_2, o[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ int least() const { return __reduce_min_sync(0xffffffffu, lim); }
+  // result [ROWS][PITCH], (maximum, sum) [ROWS][2]
+  __device__ __forceinline__ void store(float *so, float *sml, int rows, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    if (t >= rows) return;
+    if (g == 0) sml[2 * t] = m, sml[2 * t + 1] = l;
+#pragma unroll
+    for (int i = 0; i < HDP / 8; i++) {
+      const float2 v = unpair(o[i]);
+      so[t * PITCH + 8 * i + g] = v.x + v.y;
+    }
+  }
+};
+
+// Five to eight (RG = 1) or nine to sixteen rows (RG = 2): the query rows are the row operand, values in the upper and residues
+// in the lower 8 rows, codes its 8 columns: lane (g, t) has the scores of rows 8r + g at positions 8t .. 8t + 7.
+template <int HDP, int RG>
+struct ManyRows {
+  static constexpr int ROWS = 8 * RG, KS = HDP / 16, NT = HDP / 8, PITCH = HDP + 8, RESIDENT = HDP * RG <= 64 ? 4 : HDP * RG <= 128 ? 3 : 2;
+  uint32_t qf[RG][KS][4];
+  float qs[RG], m[RG], l[RG];
+  uint64_t o[RG][NT];
+  int lim[RG];
+
+  __device__ __forceinline__ void start(const AttnParams &p, int s, int h, int row0, const Sight &sight, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      const int row = row0 + r * 8 + g;
+      float x[KS][4];
+      qs[r] = load_row<KS>(p, s, h, row, t, x);
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        split2(x[k][0], x[k][1], qf[r][k][0], qf[r][k][1]);
+        split2(x[k][2], x[k][3], qf[r][k][2], qf[r][k][3]);
+      }
+      lim[r] = row < p.G * p.T ? sight.limit(row / p.G) : sight.len;
+      m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NT; i++) o[r][i] = 0;
     }
   }
 
-  bool ok = true;
-  int st = 0, parity = 0;
-  for (int b = b0; b < b1; b += kWarps) {
-    ok = __all_sync(0xffffffffu, tc::mbar_wait(bars + 8 * st, parity, p.wait_limit)) && ok;
-    const uint8_t *sb = ring + warp * (NST * BB) + st * BB;
+  // `all`: every row sees every position of the block
+  __device__ __forceinline__ void block(const uint8_t *sb, int first, bool all, int lane) {
+    const int t = lane & 3;
     float sc[RG][4][4];
 #pragma unroll
     for (int r = 0; r < RG; r++)
@@ -182,42 +315,46 @@ __global__ void __launch_bounds__(kThreads) k_attn_kv8(const AttnParams p) {
       for (int u = 0; u < 4; u++) {
         uint32_t x, y;
         widen(w[u], x, y);
+        const int j = (4 * c + u) / KS, k = (4 * c + u) % KS;
 #pragma unroll
-        for (int r = 0; r < RG; r++) mma(sc[r][(4 * c + u) / KS], qf[r][(4 * c + u) % KS], x, y);
+        for (int r = 0; r < RG; r++) mma(sc[r][j], qf[r][k][0], qf[r][k][1], qf[r][k][2], qf[r][k][3], x, y);
       }
     }
     const float2 scales = *(const float2 *)(sb + 2 * kBlock * HDP);
     uint32_t pf[RG][2][4];
-    float add[RG], old[RG];
-    bool sees[RG];
+    float add[RG];
 #pragma unroll
     for (int r = 0; r < RG; r++) {
-      const int n = lim[r] - b * kBlock - 8 * t;  // this lane's positions 0..n-1 are seen
+      const int n = lim[r] - first - 8 * t;  // this lane's positions 0..n-1 are seen
+      const float f = scales.x * kScoreUnit * qs[r];
       float v[4][2], top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          v[j][e] = (sc[r][j][e] + sc[r][j][2 + e]) * qs[r] * scales.x;
-          if (2 * j + e < n) top = fmaxf(top, v[j][e]);
+          v[j][e] = (sc[r][j][e] + sc[r][j][2 + e]) * f;
+          if (!all) v[j][e] = 2 * j + e < n ? v[j][e] : -INFINITY;
+          top = fmaxf(top, v[j][e]);
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float ref = top == -INFINITY ? 0.0f : top;
+      const float ref = top == -INFINITY ? 0.0f : top - kUp, M = fmaxf(m[r], top), c = rescale(top, M);
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          v[j][e] = 2 * j + e < n ? __expf(v[j][e] - ref) : 0.0f;
+          v[j][e] = ex2(v[j][e] - ref);
           sum += v[j][e];
         }
-      const float M = fmaxf(m[r], top);
-      sees[r] = lim[r] > b * kBlock;
-      old[r] = rescale(m[r], M);
-      const float c = rescale(top, M);
-      if (sees[r]) l[r] = l[r] * old[r] + sum * c;
-      add[r] = c * scales.y;
+      const float old = rescale(m[r], M);
+      l[r] = fmaf(l[r], old, sum * c);
+      if (__any_sync(0xffffffffu, old != 1.0f)) {
+        const uint64_t old_2 = pair(old, old);
+#pragma unroll
+        for (int i = 0; i < NT; i++) o[r][i] = mul2(o[r][i], old_2);
+      }
+      add[r] = lim[r] > first ? c * scales.y : 0.0f;  // (a block that a row sees nothing of may hold NaN)
       m[r] = M;
 #pragma unroll
       for (int kk = 0; kk < 2; kk++) {
@@ -237,105 +374,388 @@ __global__ void __launch_bounds__(kThreads) k_attn_kv8(const AttnParams p) {
 #pragma unroll
         for (int r = 0; r < RG; r++) {
           float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma(acc, pf[r][0], x0, y0);
-          mma(acc, pf[r][1], x1, y1);
-          float(&d)[2] = o[r][2 * c + u];
-          if (sees[r]) {
-            d[0] = fmaf(d[0], old[r], (acc[0] + acc[2]) * add[r]);
-            d[1] = fmaf(d[1], old[r], (acc[1] + acc[3]) * add[r]);
-          }
+          mma(acc, pf[r][0][0], pf[r][0][1], pf[r][0][2], pf[r][0][3], x0, y0);
+          mma(acc, pf[r][1][0], pf[r][1][1], pf[r][1][2], pf[r][1][3], x1, y1);
+          uint64_t &d = o[r][2 * c + u];
+          d = fma2(add2(pair(acc[0], acc[1]), pair(acc[2], acc[3])), pair(add[r], add[r]), d);
         }
       }
     }
-    __syncwarp();
-    if (lane == 0 && b + NST * kWarps < b1) fetch(b + NST * kWarps, st);
-    if (++st == NST) st = 0, parity ^= 1;
   }
-  if (!ok && lane == 0) {
-    atomicExch(p.status, 81);
-    p.status[1] = blockIdx.x, p.status[2] = warp;
-  }
-
-  // the four warps' results, then the splits'
-  float *mo = (float *)(ring + warp * (NST * BB));  // [ROWS][HDP]
+  __device__ __forceinline__ int least() const {
+    int v = lim[0];
 #pragma unroll
-  for (int r = 0; r < RG; r++) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (t == 0) sml[warp][r * 8 + g][0] = m[r], sml[warp][r * 8 + g][1] = l[r];
-#pragma unroll
-    for (int i = 0; i < NT; i++) *(float2 *)(mo + (r * 8 + g) * HDP + 8 * i + 2 * t) = make_float2(o[r][i][0], o[r][i][1]);
+    for (int r = 1; r < RG; r++) v = min(v, lim[r]);
+    return __reduce_min_sync(0xffffffffu, v);
   }
-  __syncthreads();
-  auto finish = [&](int row, int d, float M, float L, float a) {  // one value of the result
-    const int gr = rg * ROWS + row;
-    if (gr >= nrows || d >= p.HD) return;
-    const int i = gr / p.G, col = (h * p.G + gr - i * p.G) * p.HD + d, C = p.H * p.G * p.HD;
-    const float y = limit(gr) > 0 ? a / L : 0.0f;
-    const long long orow = (long long)s * p.T + i;
-    p.out[orow * C + col] = y;
-    if (p.y16) {
-      __half *d16 = p.y16 + ((long long)(col >> 6) * p.R + orow) * 64 + (col & 63);
-      const __half hi = __float2half_rn(y);
-      *d16 = hi;
-      if (p.lo_off) d16[p.lo_off] = __float2half_rn(y - __half2float(hi));
+  __device__ __forceinline__ void store(float *so, float *sml, int rows, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      const int row = r * 8 + g;
+      if (row >= rows) continue;
+      if (t == 0) sml[2 * row] = m[r], sml[2 * row + 1] = l[r];
+#pragma unroll
+      for (int i = 0; i < NT; i++) *(float2 *)(so + row * PITCH + 8 * i + 2 * t) = unpair(o[r][i]);
     }
-  };
-  const size_t part = ((size_t)unit * p.rowgroups + rg) * p.splits;
-  for (int i = threadIdx.x; i < ROWS * HDP; i += kThreads) {
-    const int row = i / HDP, d = i - row * HDP;
-    float M = -INFINITY, L = 0.0f, a = 0.0f;
+  }
+};
+
+template <int HDP>
+__host__ __device__ constexpr int stages() { return HDP <= 32 ? 8 : HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1; }
+// rings, then two results of each warp, `rows` rows each
+template <int HDP, class Acc>
+__host__ __device__ constexpr size_t smem_bytes(int rows = Acc::ROWS) {
+  return (size_t)kWarps * stages<HDP>() * kv8::block_bytes(HDP) + (size_t)2 * kWarps * rows * (Acc::PITCH + 2) * 4;
+}
+// What a unit costs a warp beside its blocks (queries, its result), in blocks: shares of the list are equal with it.
+constexpr int kTurn = 4;
+constexpr int kLeast = 2;  // places of a warp's share at least
+
+// Result row from its parts: maximum and sum of weights, channels lane, lane + 32, ...
+template <int HDP>
+struct Joined {
+  float M = -INFINITY, L = 0.0f, a[HDP / 32];
+  __device__ __forceinline__ Joined() {
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) M = fmaxf(M, sml[w][row][0]);
+    for (int i = 0; i < HDP / 32; i++) a[i] = 0.0f;
+  }
+  __device__ __forceinline__ void add(float m, float l, const float (&v)[HDP / 32]) {
+    const float top = fmaxf(M, m), f = rescale(M, top), w = rescale(m, top);
+    M = top, L = fmaf(L, f, l * w);
+#pragma unroll
+    for (int i = 0; i < HDP / 32; i++) a[i] = fmaf(a[i], f, v[i] * w);
+  }
+  __device__ __forceinline__ void finish(const AttnParams &p, int s, int h, int row, bool sees, int lane) const {
+    const int i = row / p.G, C = p.H * p.G * p.HD, col0 = (h * p.G + row - i * p.G) * p.HD;
+    const long long orow = (long long)s * p.T + i;
+    const float inv = kValueUnit / L;
+#pragma unroll
+    for (int k = 0; k < HDP / 32; k++) {
+      const int d = lane + 32 * k, col = col0 + d;
+      if (d >= p.HD) break;
+      const float y = sees ? a[k] * inv : 0.0f;
+      p.out[orow * C + col] = y;
+      if (p.y16) {
+        __half *d16 = p.y16 + ((long long)(col >> 6) * p.R + orow) * 64 + (col & 63);
+        const __half hi = __float2half_rn(y);
+        *d16 = hi;
+        if (p.lo_off) d16[p.lo_off] = __float2half_rn(y - __half2float(hi));
+      }
+    }
+  }
+};
+
+// All blocks of all units (stream, head, group of rows) form one list, of which every warp takes an equal share and streams it
+// through a ring of its own that the copy engine keeps full across the units' borders: no barrier, and no warp waits for
+// another's blocks.  A unit inside a share is finished by its warp.  The others meet first in the thread block, whose warps'
+// shares are neighbours, then, where a unit lies in several thread blocks, in the one that takes the last ticket; parts are
+// joined in the list's order (nothing waits, and the result does not depend on who comes last).
+template <int HDP, class Acc>
+__global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const AttnParams p) {
+  constexpr int BB = (int)kv8::block_bytes(HDP), NST = stages<HDP>(), ROWS = Acc::ROWS, PITCH = Acc::PITCH, NK = HDP / 32;
+  extern __shared__ __align__(128) uint8_t ring[];  // [kWarps][NST][BB], then results [2*kWarps][rows][PITCH] and [2*kWarps][rows][2]
+  __shared__ __align__(8) uint64_t full[kWarps][NST];
+  __shared__ int found[kWarps][3];      // unit, first block and unit's place in the list at the start of a warp's share
+  __shared__ int scan[kWarps];
+  __shared__ int part_unit[2 * kWarps], part_base[2 * kWarps];
+  __shared__ int open_unit[2], open_base[2], last[2];  // units that lie in other thread blocks too: before this one, behind it
+  const int nrows = p.G * p.T, rows = min(ROWS, nrows);
+  float *res = (float *)(ring + kWarps * NST * BB), *resml = res + 2 * kWarps * rows * PITCH;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < kWarps * NST) tc::mbar_init(smem_u32(&full[0][0] + threadIdx.x), 1);
+  if (threadIdx.x < 2 * kWarps) part_unit[threadIdx.x] = -1;
+  if (threadIdx.x < 2) open_unit[threadIdx.x] = -1;
+  tc::fence_barrier_init();
+  __syncthreads();
+  fa_grid_dep_sync();
+
+  Sight sight;
+  bool bad;
+  const int each = p.H * p.rowgroups;  // units of a stream
+  const bool ragged = p.lens || p.rows.pos || p.rows.counts;
+  const int shares = (int)gridDim.x * kWarps, mine = (int)blockIdx.x * kWarps + warp;
+  int total = 0, per, unit = 0, b0 = 0, base = 0;  // places, a share, its first unit, first block in that, the unit's place in the list
+  if (!ragged) {
+    sight.of(p, 0, bad);
+    const int nb = sight.blocks() + kTurn;
+    total = p.S * each * nb;
+    per = (total + shares - 1) / shares;
+    const int f0 = min(mine * per, total);
+    unit = f0 / nb, b0 = f0 - unit * nb, base = unit * nb;
+  } else {  // streams of different lengths: each thread sums a run of them, the one that holds a share's start looks closer
+    const int run = (p.S + kThreads - 1) / kThreads, s0 = min((int)threadIdx.x * run, p.S), s1 = min(s0 + run, p.S);
+    int sum = 0;
+    for (int s = s0; s < s1; s++) {
+      sight.of(p, s, bad);
+      if (bad && blockIdx.x == 0) atomicOr(p.status + 3, kStatusKv8Length);
+      sum += (sight.blocks() + kTurn) * each;
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) scan[warp] = upto;
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; w++) {
-      const float f = rescale(sml[w][row][0], M);
-      L += sml[w][row][1] * f;
-      a += *((const float *)(ring + w * (NST * BB)) + i) * f;
+      if (w < warp) upto += scan[w];
+      total += scan[w];
     }
-    if (p.splits == 1) {
-      finish(row, d, M, L, a);
-    } else {
-      p.pacc[(part + split) * ROWS * HDP + i] = a;
-      if (d == 0) *(float2 *)(p.pml + ((part + split) * ROWS + row) * 2) = make_float2(M, L);
+    per = (total + shares - 1) / shares;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+      const int f0 = ((int)blockIdx.x * kWarps + w) * per;
+      if (f0 < upto - sum || f0 >= upto) continue;
+      int at = upto - sum, s = s0;
+      for (;; s++) {
+        sight.of(p, s, bad);
+        if (f0 < at + (sight.blocks() + kTurn) * each) break;
+        at += (sight.blocks() + kTurn) * each;
+      }
+      const int nb = sight.blocks() + kTurn, h = (f0 - at) / nb;
+      found[w][0] = s * each + h, found[w][1] = f0 - at - h * nb, found[w][2] = at + h * nb;
+    }
+    __syncthreads();
+    if (mine * per < total) unit = found[warp][0], b0 = found[warp][1], base = found[warp][2];
+  }
+  if ((int)blockIdx.x * kWarps * per >= total) return;  // (the whole thread block)
+  const int f1 = min((mine + 1) * per, total);
+  auto place = [&](int u, int &s, int &h, int &row0) {
+    const int sh = u / p.rowgroups;
+    s = sh / p.H, h = sh - s * p.H, row0 = (p.rg0 + u - sh * p.rowgroups) * ROWS;
+  };
+  int s, h, row0;
+  bool ok = true;
+  if (mine * per < total) {
+    place(unit, s, h, row0);
+    sight.of(p, s, bad);
+    if (b0 >= sight.blocks()) base += sight.blocks() + kTurn, unit++, b0 = 0;  // the share begins behind a unit's blocks
+  } else {
+    base = f1;
+  }
+  if (base < f1) {
+    place(unit, s, h, row0);
+    sight.of(p, s, bad);
+    const uint32_t slots = smem_u32(ring) + warp * (NST * BB), bars = smem_u32(&full[warp][0]);
+    // the next block to fetch
+    int pu = unit, pbase = base, pnb = sight.blocks(), pleft = min(pnb, f1 - pbase) - b0, pst = 0;
+    const uint8_t *psrc = p.codes + ((size_t)(pu / p.rowgroups) * p.nblk + b0) * BB;
+    auto fetch = [&]() {  // (all lanes keep the place, one issues)
+      if (pleft == 0) {
+        pbase += pnb + kTurn, pu++;
+        if (pbase >= f1) {
+          pbase -= pnb + kTurn, pu--;
+          return;
+        }
+        if (ragged) {
+          Sight next;
+          bool b;
+          next.of(p, pu / each, b);
+          pnb = next.blocks();
+        }
+        pleft = min(pnb, f1 - pbase);
+        psrc = p.codes + (size_t)(pu / p.rowgroups) * p.nblk * BB;
+      }
+      if (lane == 0) {
+        tc::mbar_expect_tx(bars + 8 * pst, BB);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(slots + pst * BB),
+                     "l"(psrc), "r"(BB), "r"(bars + 8 * pst)
+                     : "memory");
+      }
+      psrc += BB, pleft--;
+      if (++pst == NST) pst = 0;
+    };
+#pragma unroll 1
+    for (int k = 0; k < NST; k++) fetch();
+
+    int st = 0, parity = 0;
+#pragma unroll 1
+    for (;;) {  // one unit, or the part of it in this share
+      const int nb = sight.blocks(), b1 = min(nb, f1 - base);
+      Acc acc;
+      acc.start(p, s, h, row0, sight, lane);
+      const int least = acc.least();
+#pragma unroll 1
+      for (int b = b0; b < b1; b++) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(bars + 8 * st, parity, p.wait_limit)) && ok;
+        acc.block(ring + (warp * NST + st) * BB, b * kBlock, (b + 1) * kBlock <= least, lane);
+        __syncwarp();
+        fetch();
+        if (++st == NST) st = 0, parity ^= 1;
+      }
+      const int slot = 2 * warp + (b0 == 0);  // the part in front of all others, or behind
+      float *ro = res + slot * rows * PITCH, *rm = resml + slot * rows * 2;
+      __syncwarp();
+      acc.store(ro, rm, rows, lane);
+      __syncwarp();
+      if (b0 == 0 && b1 == nb) {
+        for (int row = 0; row < min(rows, nrows - row0); row++) {
+          Joined<HDP> j;
+          float v[NK];
+#pragma unroll
+          for (int i = 0; i < NK; i++) v[i] = ro[row * PITCH + lane + 32 * i];
+          j.add(rm[2 * row], rm[2 * row + 1], v);
+          j.finish(p, s, h, row0 + row, sight.limit((row0 + row) / p.G) > 0, lane);
+        }
+      } else if (lane == 0) {
+        part_unit[slot] = unit, part_base[slot] = base;
+      }
+      base += nb + kTurn, unit++, b0 = 0;
+      if (base >= f1) break;
+      place(unit, s, h, row0);
+      sight.of(p, s, bad);
+    }
+    if (!ok && lane == 0) {
+      atomicExch(p.status, 81);
+      p.status[1] = blockIdx.x, p.status[2] = warp;
     }
   }
-  if (p.splits == 1) return;
+  __syncthreads();
+
+  // parts of the thread block's warps; a unit's parts are neighbours
+  const int share = kWarps * per, first = (int)blockIdx.x * share;
+  for (int i = 0, group = 0; i < 2 * kWarps;) {
+    const int u = part_unit[i];
+    if (u < 0) {
+      i++;
+      continue;
+    }
+    int end = i + 1;
+    while (end < 2 * kWarps && (part_unit[end] < 0 || part_unit[end] == u)) end++;
+    if ((group++ & (kWarps - 1)) == warp) {
+      const int at = part_base[i];
+      place(u, s, h, row0);
+      sight.of(p, s, bad);
+      const bool whole = at >= first && at + sight.blocks() <= first + share;
+      const int side = at >= first;
+      for (int row = 0; row < min(rows, nrows - row0); row++) {
+        Joined<HDP> j;
+        for (int k = i; k < end; k++) {
+          if (part_unit[k] < 0) continue;
+          float v[NK];
+#pragma unroll
+          for (int c = 0; c < NK; c++) v[c] = res[(k * rows + row) * PITCH + lane + 32 * c];
+          j.add(resml[(k * rows + row) * 2], resml[(k * rows + row) * 2 + 1], v);
+        }
+        if (whole) {
+          j.finish(p, s, h, row0 + row, sight.limit((row0 + row) / p.G) > 0, lane);
+        } else {
+          const size_t part = ((size_t)blockIdx.x * 2 + side) * rows + row;
+#pragma unroll
+          for (int c = 0; c < NK; c++) p.pacc[part * HDP + lane + 32 * c] = j.a[c];
+          if (lane == 0) *(float2 *)(p.pml + part * 2) = make_float2(j.M, j.L);
+        }
+      }
+      if (!whole && lane == 0) open_unit[side] = u, open_base[side] = at;
+    }
+    i = end;
+  }
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int *tk = p.tickets + (size_t)unit * p.rowgroups + rg;
-    last = atomicAdd(tk, 1) == p.splits - 1;
-    if (last) *tk = 0;  // ready for the next launch on this stream
+  if (open_unit[0] < 0 && open_unit[1] < 0) return;
+  if (threadIdx.x < 2) {
+    const int u = open_unit[threadIdx.x];
+    last[threadIdx.x] = 0;
+    if (u >= 0) {
+      place(u, s, h, row0);
+      sight.of(p, s, bad);
+      const int at = open_base[threadIdx.x], others = (at + sight.blocks() - 1) / share - at / share;
+      last[threadIdx.x] = atomicAdd(p.tickets + u, 1) == others;
+      if (last[threadIdx.x]) p.tickets[u] = 0;  // ready for the next launch on this stream
+    }
   }
   __syncthreads();
-  if (!last) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < ROWS * HDP; i += kThreads) {
-    const int row = i / HDP, d = i - row * HDP;
-    float M = -INFINITY, L = 0.0f, a = 0.0f;
-    for (int k = 0; k < p.splits; k++) M = fmaxf(M, __ldcg(p.pml + ((part + k) * ROWS + row) * 2));
-    for (int k = 0; k < p.splits; k++) {
-      const float2 ml = __ldcg((const float2 *)(p.pml + ((part + k) * ROWS + row) * 2));
-      const float f = rescale(ml.x, M);
-      L += ml.y * f;
-      a += __ldcg(p.pacc + (part + k) * ROWS * HDP + i) * f;
+  for (int k = 0; k < 2; k++) {
+    if (!last[k]) continue;
+    __threadfence();
+    const int at = open_base[k];
+    place(open_unit[k], s, h, row0);
+    sight.of(p, s, bad);
+    const int c0 = at / share, c1 = (at + sight.blocks() - 1) / share;
+    for (int row = warp; row < min(rows, nrows - row0); row += kWarps) {
+      Joined<HDP> j;
+      constexpr int kParts = HDP <= 64 ? 8 : 4;  // in flight together
+      for (int c = c0; c <= c1; c += kParts) {
+        float2 ml[kParts];
+        float v[kParts][NK];
+#pragma unroll
+        for (int n = 0; n < kParts; n++) {
+          const int cc = min(c + n, c1);
+          const size_t part = ((size_t)cc * 2 + (at >= cc * share)) * rows + row;
+          ml[n] = __ldcg((const float2 *)(p.pml + part * 2));
+#pragma unroll
+          for (int i = 0; i < NK; i++) v[n][i] = __ldcg(p.pacc + part * HDP + lane + 32 * i);
+        }
+#pragma unroll
+        for (int n = 0; n < kParts; n++)
+          if (c + n <= c1) j.add(ml[n].x, ml[n].y, v[n]);
+      }
+      j.finish(p, s, h, row0 + row, sight.limit((row0 + row) / p.G) > 0, lane);
     }
-    finish(row, d, M, L, a);
   }
 }
 
-template <int HDP, int RG>
-cudaError_t launch(fa_ctx *ctx, const AttnParams &p, int grid) {
-  static SmemLimit limit;
-  constexpr size_t smem = (size_t)kWarps * stages<HDP>() * kv8::block_bytes(HDP);
-  const cudaError_t e = limit.raise(ctx, k_attn_kv8<HDP, RG>, smem);
-  if (e != cudaSuccess) return e;
-  return fa_launch_dep(ctx, k_attn_kv8<HDP, RG>, dim3(grid), dim3(kThreads), smem, p);
+// Resident thread blocks per SM of a kernel, asked once.
+template <int HDP, class Acc>
+int resident(int rows) {
+  static std::atomic<int> asked[Acc::ROWS];
+  auto &known = asked[rows - 1];
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_attn_kv8<HDP, Acc>, kThreads, smem_bytes<HDP, Acc>(rows)) != cudaSuccess || n < 1) n = 1;
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
+
+template <int HDP, class Acc>
+int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label) {
+  constexpr int ROWS = Acc::ROWS;
+  static SmemLimit limit;
+  FA_CHECK_CUDA(ctx, limit.raise(ctx, k_attn_kv8<HDP, Acc>, smem_bytes<HDP, Acc>()));
+  const int nb = ceil_div(most < 1 ? 1 : most, kBlock), groups = ceil_div(p.G * p.T, ROWS);
+  const long long list = (long long)c->S * c->H * (nb + kTurn);  // places of a row group, < 2^31: the cache fits the device
+  const int rows = p.G * p.T < ROWS ? p.G * p.T : ROWS, slots = ctx->sm_count * resident<HDP, Acc>(rows);
+  int rc = FA_OK;
+  for (p.rg0 = 0; p.rg0 < groups && rc == FA_OK; p.rg0 += p.rowgroups) {
+    const long long fit = 0x7fffffffLL / list;
+    p.rowgroups = (int)(groups - p.rg0 < fit ? groups - p.rg0 : fit);
+    const long long share = (list * p.rowgroups + kWarps * kLeast - 1) / (kWarps * kLeast);
+    const int grid = (int)(share < slots ? share : slots);
+    const size_t part = (size_t)grid * 2 * rows, tickets = p.rowgroups > 1 ? (size_t)c->S * c->H * p.rowgroups : 0;
+    void *scratch = nullptr;
+    size_t bytes = 0;
+    FA_TRY(fa_block_acquire(ctx, part * (HDP + 2) * 4 + tickets * 4, &scratch, &bytes));
+    p.pacc = (float *)scratch, p.pml = p.pacc + part * HDP;
+    p.tickets = c->tickets;
+    cudaError_t e = cudaSuccess;
+    if (tickets) {
+      p.tickets = (int *)(p.pml + part * 2);
+      e = cudaMemsetAsync(p.tickets, 0, tickets * 4, ctx->stream);
+    }
+    if (e == cudaSuccess) {
+      LaunchScope ls(ctx, label);
+      e = fa_launch_dep(ctx, k_attn_kv8<HDP, Acc>, dim3(grid), dim3(kThreads), smem_bytes<HDP, Acc>(rows), p);
+    }
+    if (e != cudaSuccess) rc = fa_fail(ctx, FA_ERR_CUDA, "launch %s: %s", label, cudaGetErrorString(e));
+    fa_block_release(ctx, scratch);
+  }
+  return rc;
+}
+
 template <int HDP>
-cudaError_t launch(fa_ctx *ctx, const AttnParams &p, int rgroups, int grid) {
-  return rgroups == 1 ? launch<HDP, 1>(ctx, p, grid) : launch<HDP, 2>(ctx, p, grid);
+int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label) {
+  const int rows = p.G * p.T;
+  if (rows <= 4) return run<HDP, FewRows<HDP>>(ctx, c, p, most, label);
+  if constexpr (HDP <= 128) {  // (16 rows of 256 do not fit the registers)
+    if (rows > 8) return run<HDP, ManyRows<HDP, 2>>(ctx, c, p, most, label);
+  }
+  return run<HDP, ManyRows<HDP, 1>>(ctx, c, p, most, label);
 }
 
 // Attention of p's queries over the cache, whose positions end at `most` at the latest; the result is [S*T][H*G*HD].
@@ -348,7 +768,7 @@ int attend(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *la
     return FA_OK;
   }
   p.out = (float *)y->dptr, p.R = y->rows;
-  p.codes = c->codes, p.H = c->H, p.HD = c->HD, p.nblk = c->nblk;
+  p.codes = c->codes, p.S = c->S, p.H = c->H, p.HD = c->HD, p.nblk = c->nblk;
   p.vec = c->HD % 4 == 0 && p.ldq % 4 == 0 && ((uintptr_t)p.q & 15) == 0;
   p.status = ctx->dev_status, p.wait_limit = ctx->wait_limit;
   if ((C & 63) == 0 && fa_tc_available(ctx)) {  // the product that follows reads the packed operand
@@ -359,32 +779,9 @@ int attend(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *la
     }
     if (p.y16) y->a16_valid = true;
   }
-  const int rgroup = p.G * p.T > 8 && c->HDP <= 128 ? 2 : 1, nb = ceil_div(most < 1 ? 1 : most, kBlock);
-  p.rowgroups = ceil_div(p.G * p.T, 8 * rgroup);
-  const long long units = (long long)c->S * c->H * p.rowgroups;
-  long long splits = (4ll * ctx->sm_count + units - 1) / units;
-  if (splits > ceil_div(nb, kWarps)) splits = ceil_div(nb, kWarps);
-  if (units > ctx->gemv_ticket_count) splits = 1;
-  p.kper = ceil_div(ceil_div(nb, (int)splits), kWarps) * kWarps;
-  p.splits = ceil_div(nb, p.kper);
-  void *scratch = nullptr;
-  size_t bytes = 0;
-  int rc = FA_OK;
-  if (units * p.splits > 0x7fffffffLL) rc = fa_fail(ctx, FA_ERR_INVALID, "%s: too many rows in one call", label);
-  if (rc == FA_OK && p.splits > 1) {
-    const size_t n = (size_t)units * p.splits * 8 * rgroup;
-    rc = fa_block_acquire(ctx, n * c->HDP * 4 + n * 8, &scratch, &bytes);
-    p.pacc = (float *)scratch, p.pml = (float *)scratch + n * c->HDP, p.tickets = ctx->gemv_tickets;
-  }
-  if (rc == FA_OK) {
-    LaunchScope ls(ctx, label);
-    const int grid = (int)(units * p.splits);
-    const cudaError_t e = c->HDP == 32 ? launch<32>(ctx, p, rgroup, grid) : c->HDP == 64 ? launch<64>(ctx, p, rgroup, grid)
-                        : c->HDP == 96 ? launch<96>(ctx, p, rgroup, grid) : c->HDP == 128 ? launch<128>(ctx, p, rgroup, grid)
-                                       : launch<256, 1>(ctx, p, grid);
-    if (e != cudaSuccess) rc = fa_fail(ctx, FA_ERR_CUDA, "launch %s: %s", label, cudaGetErrorString(e));
-  }
-  if (scratch) fa_block_release(ctx, scratch);
+  const int rc = c->HDP == 32 ? run<32>(ctx, c, p, most, label) : c->HDP == 64 ? run<64>(ctx, c, p, most, label)
+               : c->HDP == 96 ? run<96>(ctx, c, p, most, label) : c->HDP == 128 ? run<128>(ctx, c, p, most, label)
+                              : run<256>(ctx, c, p, most, label);
   if (rc != FA_OK) {
     fa_free_tensor(ctx, y);
     return rc;

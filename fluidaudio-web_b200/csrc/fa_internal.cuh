@@ -91,6 +91,7 @@ struct fa_kv8 {
   uint8_t *codes = nullptr;         // [S][H][nblk] blocks
   float *tail = nullptr;            // [S][H][2][32][HD]: f32 rows of the block that was written last, keys then values
   int *tag = nullptr;               // [S][H][2]: which block that is
+  int *tickets = nullptr;           // [S][H] arrival counters of the attention's parts, zero between launches
 };
 
 struct fa_staged {

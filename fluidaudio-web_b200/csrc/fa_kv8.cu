@@ -60,8 +60,8 @@ __device__ __forceinline__ float stored(const uint8_t *blk, int which, int pos, 
   } else {
     lane = (ch & 7) * 4 + (pos >> 3), wi = (ch >> 3) * 2 + ((pos & 7) >> 2), e = pos & 3;
   }
-  const uint8_t u = blk[(size_t)which * kBlock * HDP + (wi >> 2) * 512 + lane * 16 + (wi & 3) * 4 + e];
-  return (float)((int)u - 128) * ((const float *)(blk + (size_t)2 * kBlock * HDP))[which];
+  const uint32_t w = *(const uint32_t *)(blk + (size_t)which * kBlock * HDP + (wi >> 2) * 512 + lane * 16 + (wi & 3) * 4);
+  return kv8::unpack(w, e) * ((const float *)(blk + (size_t)2 * kBlock * HDP))[which];
 }
 
 // One (stream, head, keys or values): the thread block of x == 0 takes the first and the last block that the rows touch, one
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_write(const WriteParams p) {
 #pragma unroll
           for (int e = 0; e < 4; e++) q[e] = code_of(sx[(pos + e) * pitch + ch], scale, inv);
         }
-        w[u] = (uint32_t)(q[0] + 128) | (uint32_t)(q[1] + 128) << 8 | (uint32_t)(q[2] + 128) << 16 | (uint32_t)(q[3] + 128) << 24;
+        w[u] = kv8::pack4(q);
       }
       *(uint4 *)(blk + (size_t)which * kBlock * HDP + (size_t)c * 512 + ln * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -165,7 +165,7 @@ struct ReadParams {
 };
 
 __global__ void __launch_bounds__(kThreads) k_kv8_read(const ReadParams p) {
-  extern __shared__ uint8_t sb[];  // half a block
+  extern __shared__ __align__(16) uint8_t sb[];  // half a block
   fa_grid_dep_sync();
   const int h = blockIdx.y >> 1, which = blockIdx.y & 1, s = blockIdx.z, HD = p.HD, HDP = p.HDP;
   const int b = p.row0 / kBlock + blockIdx.x, half = kBlock * HDP;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) k_kv8_read(const ReadParams p) {
     int lane, wi, e;
     if (which == 0) lane = ((r >> 3) * 2 + (r & 1)) * 4 + ((d & 15) >> 2), wi = ((r & 7) >> 1) * KS + (d >> 4), e = d & 3;
     else lane = (d & 7) * 4 + (r >> 3), wi = (d >> 3) * 2 + ((r & 7) >> 2), e = r & 3;
-    out[(size_t)r * p.H * HD + d] = (float)((int)sb[(wi >> 2) * 512 + lane * 16 + (wi & 3) * 4 + e] - 128) * scale;
+    out[(size_t)r * p.H * HD + d] = kv8::unpack(*(const uint32_t *)(sb + (wi >> 2) * 512 + lane * 16 + (wi & 3) * 4), e) * scale;
   }
 }
 
@@ -199,16 +199,18 @@ extern "C" int fa_kv8_create(fa_ctx *ctx, int S, int positions, int H, int HD, f
   c.S = S, c.P = positions, c.H = H, c.HD = HD;
   c.HDP = kv8::stored_width(HD), c.nblk = ceil_div(positions, kBlock);
   const size_t units = (size_t)S * H;
-  const size_t codes = units * c.nblk * kv8::block_bytes(c.HDP), tail = units * 2 * kBlock * HD * 4, tag = units * 2 * 4;
+  const size_t codes = units * c.nblk * kv8::block_bytes(c.HDP), tail = units * 2 * kBlock * HD * 4, tag = units * 2 * 4, tickets = units * 4;
   size_t blk = 0;
   int rc = fa_block_acquire(ctx, codes, (void **)&c.codes, &blk);
   if (rc == FA_OK) rc = fa_block_acquire(ctx, tail, (void **)&c.tail, &blk);
   if (rc == FA_OK) rc = fa_block_acquire(ctx, tag, (void **)&c.tag, &blk);
+  if (rc == FA_OK) rc = fa_block_acquire(ctx, tickets, (void **)&c.tickets, &blk);
   // zero codes with zero scales: a position that nothing was written to reads as zeros; no tail holds a block yet
-  if (rc == FA_OK && (cudaMemsetAsync(c.codes, 0, codes, ctx->stream) != cudaSuccess || cudaMemsetAsync(c.tag, 0xff, tag, ctx->stream) != cudaSuccess))
+  if (rc == FA_OK && (cudaMemsetAsync(c.codes, 0, codes, ctx->stream) != cudaSuccess || cudaMemsetAsync(c.tag, 0xff, tag, ctx->stream) != cudaSuccess ||
+                      cudaMemsetAsync(c.tickets, 0, tickets, ctx->stream) != cudaSuccess))
     rc = fa_fail(ctx, FA_ERR_CUDA, "kvCache8: %s", cudaGetErrorString(cudaGetLastError()));
   if (rc != FA_OK) {
-    for (void *q : {(void *)c.codes, (void *)c.tail, (void *)c.tag})
+    for (void *q : {(void *)c.codes, (void *)c.tail, (void *)c.tag, (void *)c.tickets})
       if (q) fa_block_release(ctx, q);
     return rc;
   }
@@ -224,6 +226,7 @@ extern "C" int fa_kv8_free(fa_ctx *ctx, fa_kv8 *c) {
   fa_block_release(ctx, c->codes);
   fa_block_release(ctx, c->tail);
   fa_block_release(ctx, c->tag);
+  fa_block_release(ctx, c->tickets);
   ctx->kv8s.erase(c);
   delete c;
   return FA_OK;

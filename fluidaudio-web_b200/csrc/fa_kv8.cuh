@@ -1,8 +1,13 @@
 // The 8-bit key and value cache: layout and device helpers shared by the kernels that write and read it.
 //
 // A block holds 32 consecutive positions of one head of one stream: K 32 x HDP codes, V 32 x HDP codes, then the two scales.
-// A code is u = q + 128 with q = rint(x / scale) in -127..127 and scale = max|x| / 127 over the rows that the block holds, so
-// x is read as (u - 128) * scale: one rounding, half a step of the block's largest value / 127 at most.
+// A code is q = rint(x / scale) in -127..127 with scale = max|x| / 127 over the rows that the block holds, so x is read as
+// q * scale: one rounding, half a step of the block's largest value / 127 at most.
+//
+// Codes are signs and magnitudes, four to a word in an order that makes them f16 operands with three instructions: an f16 with
+// a zero exponent is a whole number times 2^-24, so sign (bit 15) and magnitude (bits 0..6) ARE the code.  Each half of a word
+// holds one code that way, and a second one with its sign in bit 7 and its magnitude in bits 8..14, which is the first kind
+// once the half's bytes change places: codes 0 and 1 of the word are the halves' first, 2 and 3 their second ones.
 //
 // The codes lie in the order in which the lanes of a warp take them as operands of m16n8k16 products (B fragments: lane
 // (g, t) = (lane / 4, lane % 4) holds column g and k = 2t, 2t+1, 2t+8, 2t+9), 16 bytes a lane and 512 a warp:
@@ -31,6 +36,21 @@ __device__ __forceinline__ void k_place(int wi, int lane, int KS, int &pos, int 
 __device__ __forceinline__ void v_place(int wi, int lane, int &pos, int &ch) {
   const int g = lane >> 2, t = lane & 3;
   pos = 8 * t + 4 * (wi & 1), ch = 8 * (wi >> 1) + g;  // positions pos..pos+3
+}
+
+__device__ __forceinline__ uint32_t pack4(const int (&q)[4]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const uint32_t sign = q[e] < 0, mag = (uint32_t)abs(q[e]);
+    w |= e < 2 ? (mag | sign << 15) << (16 * e) : (mag << 8 | sign << 7) << (16 * (e - 2));
+  }
+  return w;
+}
+// code e of a word
+__device__ __forceinline__ float unpack(uint32_t w, int e) {
+  const uint32_t half = w >> (16 * (e & 1)), mag = half >> (e < 2 ? 0 : 8) & 0x7f, sign = half >> (e < 2 ? 15 : 7) & 1;
+  return sign ? -(float)mag : (float)mag;
 }
 
 // Where stream s's new rows go: `start` = pos[s] or n, `count` = counts[s] or T rows, both inside the cache.
