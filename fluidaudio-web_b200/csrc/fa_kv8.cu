@@ -16,43 +16,19 @@ using kv8::kBlock;
 constexpr int kThreads = 128;
 
 struct WriteParams {
-  const void *src[2];  // keys, values: row (s, i) of head h at src + (s*T + i)*ld + h*HD
+  const void *keys, *values;  // row (s, i) of head h at + (s*T + i)*ld + h*HD
   long long ld;
   uint8_t *codes;
   float *tail;
   int *tag;
   kv8::Rows rows;
-  int H, HD, HDP, nblk;
+  int H, HD, nblk;
   int vec;  // rows may be read four values at a time
   int *status;
 };
 
-// rint(x / scale), the quotient exact where it matters: the product with 1 / scale is off by less than 2.4e-5 at |q| <= 127,
-// so only values that close to a tie (about one in 20000), and scales whose reciprocal overflows, take the f64 quotient,
-// which never rounds across a tie (x and scale have 24 bits each).
-__device__ __forceinline__ int code_of(float x, float scale, float inv) {
-  if (!(scale > 0.0f) || scale == INFINITY) return 0;
-  const float t = x * inv;
-  float q = rintf(t);
-  if (!(fabsf(t - q) < 0.49997f)) q = (float)rint((double)x / (double)scale);
-  return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-
-template <typename T>
-__device__ __forceinline__ float4 load4(const T *p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float *p) { return __ldcs((const float4 *)p); }
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half *p) {
-  const uint2 w = __ldcs((const uint2 *)p);
-  const float2 a = __half22float2(*(const __half2 *)&w.x), b = __half22float2(*(const __half2 *)&w.y);
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float load1(const float *p) { return *p; }
-__device__ __forceinline__ float load1(const __half *p) { return __half2float(*p); }
-
 // One value of a stored block.
-__device__ __forceinline__ float stored(const uint8_t *blk, int which, int pos, int ch, int HDP) {
+__device__ __noinline__ float stored(const uint8_t *blk, int which, int pos, int ch, int HDP) {
   int lane, wi, e;
   if (which == 0) {
     const int KS = HDP >> 4;
@@ -64,15 +40,177 @@ __device__ __forceinline__ float stored(const uint8_t *blk, int which, int pos, 
   return kv8::unpack(w, e) * ((const float *)(blk + (size_t)2 * kBlock * HDP))[which];
 }
 
+// Four neighbouring values of a row, zeros from HD on.
+__device__ __forceinline__ float4 load4(const float *p) { return __ldcs((const float4 *)p); }
+__device__ __forceinline__ float4 load4(const __half *p) {
+  const uint2 w = __ldcs((const uint2 *)p);
+  const float2 a = __half22float2(*(const __half2 *)&w.x), b = __half22float2(*(const __half2 *)&w.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float load1(const float *p) { return *p; }
+__device__ __forceinline__ float load1(const __half *p) { return __half2float(*p); }
+
+__device__ __noinline__ uint32_t exact_code(float x, float scale) {
+  return scale > 0.0f && scale < INFINITY ? (uint32_t)min(rint(fabs((double)x) / (double)scale), 127.0) : 0u;
+}
+
+// The word of four values.  The quotient's integer is taken from the product with 1 / scale, off by less than 2.4e-5 at most
+// 127; only values that close to a tie (about one in 20000), and scales whose reciprocal overflows or that are no numbers,
+// take the f64 quotient, which never rounds across a tie (x and scale have 24 bits each).
+__device__ __forceinline__ uint32_t code4(float x0, float x1, float x2, float x3, float scale, float inv) {
+  const float x[4] = {x0, x1, x2, x3};
+  uint32_t u[4];
+  float off = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float a = fabsf(x[e]) * inv, r = a + 8388608.0f;  // 2^23: the sum's low bits are the nearest integer, ties to even
+    u[e] = __float_as_uint(r);
+    off = fmaxf(off, fabsf(a - (r - 8388608.0f)));
+  }
+  if (!(off < 0.49997f) || !(scale > 1e-30f && scale < INFINITY)) {
+#pragma unroll 1
+    for (int e = 0; e < 4; e++) {
+      const uint32_t q = exact_code(e < 2 ? (e == 0 ? x0 : x1) : (e == 2 ? x2 : x3), scale);
+      if (e == 0) u[0] = q;
+      if (e == 1) u[1] = q;
+      if (e == 2) u[2] = q;
+      if (e == 3) u[3] = q;
+    }
+  }
+  const uint32_t mag = __byte_perm(__byte_perm(u[0], u[2], 0x0040), __byte_perm(u[1], u[3], 0x0040), 0x5410);
+  const uint32_t sign = __byte_perm(__byte_perm(__float_as_uint(x[2]), __float_as_uint(x[0]), 0x0073),
+                                    __byte_perm(__float_as_uint(x[3]), __float_as_uint(x[1]), 0x0073), 0x5410);
+  return mag | (sign & 0x80808080u);
+}
+
+// One block, keys (WHICH = 0) or values (1): rows to registers, their largest magnitude, codes to shared memory in the block's
+// order, from there 16 bytes a thread.  A thread takes four neighbouring channels of a row of keys, since those are one word,
+// and four by four values, whose words are four positions of a channel.
+template <typename T, int HDP, int WHICH>
+__device__ __forceinline__ void write_block(const WriteParams &p, const T *src, float *tail, uint8_t *blk, int *tag, int b, int held, int rows,
+                                            bool is_last, uint32_t *sw, uint32_t *smax) {
+  constexpr int N4 = HDP / 4, ITEMS = WHICH ? (2 * HDP + kThreads - 1) / kThreads * 4 : HDP / 16;
+  const int HD = p.HD;
+  const bool kept = held > 0 && *tag == b;  // (read before the barrier in front of its update)
+  float4 x[ITEMS];
+  auto at = [&](int k, int &r, int &d) {  // row and channel of the k-th four values
+    if (WHICH == 0) {
+      const int i = threadIdx.x + k * kThreads;
+      r = i / N4, d = (i - r * N4) * 4;
+    } else {
+      const int i = threadIdx.x + (k >> 2) * kThreads;
+      r = i / N4, d = (i - r * N4) * 4;
+      r = r * 4 + (k & 3);
+    }
+  };
+  uint32_t top = 0;  // as bits: infinities and NaNs are above all others
+#pragma unroll
+  for (int k = 0; k < ITEMS; k++) {
+    int r, d;
+    at(k, r, d);
+    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r >= held && r < rows && d < HD) {
+      const T *q = src + (long long)r * p.ld + d;
+      if (p.vec) {
+        x[k] = load4(q);
+      } else {
+        x[k].x = load1(q);
+        if (d + 1 < HD) x[k].y = load1(q + 1);
+        if (d + 2 < HD) x[k].z = load1(q + 2);
+        if (d + 3 < HD) x[k].w = load1(q + 3);
+      }
+    }
+  }
+  if (kept) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+      int r, d;
+      at(k, r, d);
+      if (r >= held || d >= HD) continue;
+      const float *q = tail + r * HD + d;
+      if (HD % 4 == 0) {
+        x[k] = *(const float4 *)q;
+      } else {
+        x[k].x = q[0];
+        if (d + 1 < HD) x[k].y = q[1];
+        if (d + 2 < HD) x[k].z = q[2];
+        if (d + 3 < HD) x[k].w = q[3];
+      }
+    }
+  } else if (held > 0) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+      int r, d;
+      at(k, r, d);
+      if (r >= held || d >= HD) continue;
+      x[k].x = stored(blk, WHICH, r, d, HDP);
+      if (d + 1 < HD) x[k].y = stored(blk, WHICH, r, d + 1, HDP);
+      if (d + 2 < HD) x[k].z = stored(blk, WHICH, r, d + 2, HDP);
+      if (d + 3 < HD) x[k].w = stored(blk, WHICH, r, d + 3, HDP);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; k++)
+    top = max(max(top, max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu)),
+              max(__float_as_uint(x[k].z) & 0x7fffffffu, __float_as_uint(x[k].w) & 0x7fffffffu));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) smax[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; w++) top = max(top, smax[w]);
+  const float scale = __uint_as_float(top) / 127.0f, inv = 1.0f / scale;
+  if (WHICH == 0) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+      int r, d;
+      at(k, r, d);
+      const int lane = ((r >> 3) * 2 + (r & 1)) * 4 + ((d & 15) >> 2), wi = ((r & 7) >> 1) * (HDP / 16) + (d >> 4);
+      sw[(wi >> 2) * 128 + lane * 4 + (wi & 3)] = code4(x[k].x, x[k].y, x[k].z, x[k].w, scale, inv);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < ITEMS; k += 4) {
+      int r, d;
+      at(k, r, d);
+      if (r >= kBlock) break;
+      uint32_t *w = sw + (d >> 4) * 128 + ((d & 7) * 4 + (r >> 3)) * 4 + (d >> 3 & 1) * 2 + ((r & 7) >> 2);  // channel d's; the next 16 on
+      w[0] = code4(x[k].x, x[k + 1].x, x[k + 2].x, x[k + 3].x, scale, inv);
+      w[16] = code4(x[k].y, x[k + 1].y, x[k + 2].y, x[k + 3].y, scale, inv);
+      w[32] = code4(x[k].z, x[k + 1].z, x[k + 2].z, x[k + 3].z, scale, inv);
+      w[48] = code4(x[k].w, x[k + 1].w, x[k + 2].w, x[k + 3].w, scale, inv);
+    }
+  }
+  if (is_last) {  // its f32 rows stay: a row that joins the block codes it anew
+#pragma unroll
+    for (int k = 0; k < ITEMS; k++) {
+      int r, d;
+      at(k, r, d);
+      if (r >= rows || (r < held && kept)) continue;
+      float *q = tail + r * HD + d;
+      if (d >= HD) continue;
+      if (HD % 4 == 0) {
+        *(float4 *)q = x[k];
+      } else {
+        q[0] = x[k].x;
+        if (d + 1 < HD) q[1] = x[k].y;
+        if (d + 2 < HD) q[2] = x[k].z;
+        if (d + 3 < HD) q[3] = x[k].w;
+      }
+    }
+    if (threadIdx.x == 0) *tag = b;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * HDP; i += kThreads) ((uint4 *)(blk + (size_t)WHICH * kBlock * HDP))[i] = ((const uint4 *)sw)[i];
+  if (threadIdx.x == 0) ((float *)(blk + (size_t)2 * kBlock * HDP))[WHICH] = scale;
+}
+
 // One (stream, head, keys or values): the thread block of x == 0 takes the first and the last block that the rows touch, one
 // after the other, since the first may need the tail that the last one replaces; the others take one block in between.
-//
-// Bound by HBM: 4 bytes in, 1 out.  The rows are staged in shared memory so that both the reads (rows) and the writes (the
-// fragment order, 16 bytes a lane) are whole sectors; 8 to 16 thread blocks an SM keep 8 KB of loads each in flight.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) k_kv8_write(const WriteParams p) {
-  extern __shared__ float sx[];  // [32][HDP + pad]
-  __shared__ float wmax[kThreads / 32];
+// Bound by HBM: 4 bytes in, 1 out.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kThreads, HDP <= 64 ? 8 : HDP <= 128 ? 5 : 3) k_kv8_write(const WriteParams p) {
+  __shared__ __align__(16) uint32_t sw[8 * HDP];
+  __shared__ uint32_t smax[kThreads / 32];
   fa_grid_dep_sync();
   const int h = blockIdx.y >> 1, which = blockIdx.y & 1, s = blockIdx.z;
   int start, count;
@@ -81,106 +219,86 @@ __global__ void __launch_bounds__(kThreads) k_kv8_write(const WriteParams p) {
   if (bad && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) atomicOr(p.status + 3, kStatusKv8Length);
   if (count <= 0) return;
   const int end = start + count, first = start / kBlock, last = (end - 1) / kBlock;
-  const int HD = p.HD, HDP = p.HDP, pitch = HDP + 1;  // odd: the values' order reads columns
   const size_t unit = (size_t)s * p.H + h;
-  float *tail = p.tail + (unit * 2 + which) * kBlock * HD;
-  const T *src = (const T *)p.src[which] + ((size_t)s * p.rows.T - start) * p.ld + (size_t)h * HD;  // + position * ld
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float *tail = p.tail + (unit * 2 + which) * kBlock * p.HD;
+  const T *src = (const T *)(which ? p.values : p.keys) + ((long long)s * p.rows.T - start) * p.ld + h * p.HD;  // + position * ld
   const int turns = blockIdx.x == 0 ? 1 + (last > first) : (int)blockIdx.x < last - first;
   for (int turn = 0; turn < turns; turn++) {
     const int b = blockIdx.x == 0 ? (turn ? last : first) : first + (int)blockIdx.x, base = b * kBlock;
     uint8_t *blk = p.codes + (unit * p.nblk + b) * kv8::block_bytes(HDP);
-    const int held = max(0, start - base);              // rows of this block from before the call
-    const int rows = min(kBlock, end - base);
-    const bool kept = held > 0 && p.tag[unit * 2 + which] == b;  // (read before the barrier in front of its update)
-    float top = 0.0f;
-    bool nan = false;
-    auto put = [&](int r, int d, float x) {
-      sx[r * pitch + d] = x;
-      top = fmaxf(top, fabsf(x));
-      nan |= x != x;
-    };
-    if (p.vec) {
-      const int n4 = HDP / 4;
-      for (int i = threadIdx.x; i < kBlock * n4; i += kThreads) {
-        const int r = i / n4, d = (i - r * n4) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rows && d < HD) {
-          if (r >= held) x = load4(src + (size_t)(base + r) * p.ld + d);
-          else if (kept) x = *(const float4 *)(tail + r * HD + d);
-          else x = make_float4(stored(blk, which, r, d, HDP), stored(blk, which, r, d + 1, HDP), stored(blk, which, r, d + 2, HDP), stored(blk, which, r, d + 3, HDP));
-        }
-        put(r, d, x.x), put(r, d + 1, x.y), put(r, d + 2, x.z), put(r, d + 3, x.w);
-      }
-    } else {
-      for (int i = threadIdx.x; i < kBlock * HDP; i += kThreads) {
-        const int r = i / HDP, d = i - r * HDP;
-        float x = 0.0f;
-        if (r < rows && d < HD) x = r >= held ? load1(src + (size_t)(base + r) * p.ld + d) : kept ? tail[r * HD + d] : stored(blk, which, r, d, HDP);
-        put(r, d, x);
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) wmax[warp] = top;
-    const bool any_nan = __syncthreads_or(nan);
-    top = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    const float scale = any_nan ? __int_as_float(0x7fc00000) : top / 127.0f, inv = 1.0f / scale;
-    const int words = HDP / 4, KS = HDP / 16;
-    for (int i = threadIdx.x; i < words * 8; i += kThreads) {  // 16 bytes: words 4c .. 4c+3 of a lane
-      const int ln = i & 31, c = i >> 5;
-      uint32_t w[4];
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        int pos, ch, q[4];
-        if (which == 0) {
-          kv8::k_place(4 * c + u, ln, KS, pos, ch);
-#pragma unroll
-          for (int e = 0; e < 4; e++) q[e] = code_of(sx[pos * pitch + ch + e], scale, inv);
-        } else {
-          kv8::v_place(4 * c + u, ln, pos, ch);
-#pragma unroll
-          for (int e = 0; e < 4; e++) q[e] = code_of(sx[(pos + e) * pitch + ch], scale, inv);
-        }
-        w[u] = kv8::pack4(q);
-      }
-      *(uint4 *)(blk + (size_t)which * kBlock * HDP + (size_t)c * 512 + ln * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    if (threadIdx.x == 0) ((float *)(blk + (size_t)2 * kBlock * HDP))[which] = scale;
-    if (b == last) {  // its f32 rows stay: a row that joins the block codes it anew
-      for (int i = threadIdx.x; i < rows * HD; i += kThreads) {
-        const int r = i / HD, d = i - r * HD;
-        if (r >= held || !kept) tail[i] = sx[r * pitch + d];
-      }
-      if (threadIdx.x == 0) p.tag[unit * 2 + which] = b;
-    }
+    const int held = max(0, start - base), rows = min(kBlock, end - base);  // rows from before the call, and in all
+    if (which == 0) write_block<T, HDP, 0>(p, src + (long long)base * p.ld, tail, blk, p.tag + unit * 2, b, held, rows, b == last, sw, smax);
+    else write_block<T, HDP, 1>(p, src + (long long)base * p.ld, tail, blk, p.tag + unit * 2 + 1, b, held, rows, b == last, sw, smax);
     __syncthreads();
   }
 }
 
+template <typename T>
+cudaError_t launch_write(fa_ctx *ctx, const WriteParams &p, dim3 grid, int HDP) {
+  auto kernel = HDP == 32 ? k_kv8_write<T, 32> : HDP == 64 ? k_kv8_write<T, 64> : HDP == 96 ? k_kv8_write<T, 96>
+              : HDP == 128 ? k_kv8_write<T, 128> : k_kv8_write<T, 256>;
+  return fa_launch_dep(ctx, kernel, grid, dim3(kThreads), 0, p);
+}
+
 struct ReadParams {
   const uint8_t *codes;
-  float *out[2];
-  int row0, rows, H, HD, HDP, nblk;
+  float *keys, *values;
+  int row0, rows, H, HD, nblk;
 };
 
+// A word of codes as four values: the codes come as f16 subnormals, whole numbers after the exact product with 2^24.
+__device__ __forceinline__ float4 values4(uint32_t w, float scale) {
+  const uint32_t a = w & 0x807F807Fu, b = __byte_perm(w, 0u, 0x2301) & 0x807F807Fu;
+  const float2 x = __half22float2(*(const __half2 *)&a), y = __half22float2(*(const __half2 *)&b);
+  return make_float4(x.x * 16777216.0f * scale, x.y * 16777216.0f * scale, y.x * 16777216.0f * scale, y.y * 16777216.0f * scale);
+}
+
+// One half of a block: a thread turns one word of keys, or four words of values, into four values of a row, or of four rows.
+template <int HDP>
 __global__ void __launch_bounds__(kThreads) k_kv8_read(const ReadParams p) {
-  extern __shared__ __align__(16) uint8_t sb[];  // half a block
+  constexpr int N4 = HDP / 4;
   fa_grid_dep_sync();
-  const int h = blockIdx.y >> 1, which = blockIdx.y & 1, s = blockIdx.z, HD = p.HD, HDP = p.HDP;
-  const int b = p.row0 / kBlock + blockIdx.x, half = kBlock * HDP;
+  const int h = blockIdx.y >> 1, which = blockIdx.y & 1, s = blockIdx.z, HD = p.HD;
+  const int b = p.row0 / kBlock + blockIdx.x;
   const uint8_t *blk = p.codes + (((size_t)s * p.H + h) * p.nblk + b) * kv8::block_bytes(HDP);
-  for (int i = threadIdx.x; i < half / 16; i += kThreads) ((uint4 *)sb)[i] = ((const uint4 *)(blk + (size_t)which * half))[i];
-  const float scale = ((const float *)(blk + (size_t)2 * half))[which];
-  __syncthreads();
-  const int KS = HDP >> 4, lo = max(p.row0 - b * kBlock, 0), hi = min(kBlock, p.row0 + p.rows - b * kBlock);
-  float *out = p.out[which] + ((size_t)s * p.rows + (size_t)b * kBlock - p.row0) * p.H * HD + (size_t)h * HD;
-  for (int i = threadIdx.x; i < (hi - lo) * HD; i += kThreads) {
-    const int r = lo + i / HD, d = i % HD;
-    int lane, wi, e;
-    if (which == 0) lane = ((r >> 3) * 2 + (r & 1)) * 4 + ((d & 15) >> 2), wi = ((r & 7) >> 1) * KS + (d >> 4), e = d & 3;
-    else lane = (d & 7) * 4 + (r >> 3), wi = (d >> 3) * 2 + ((r & 7) >> 2), e = r & 3;
-    out[(size_t)r * p.H * HD + d] = kv8::unpack(*(const uint32_t *)(sb + (wi >> 2) * 512 + lane * 16 + (wi & 3) * 4), e) * scale;
+  const uint32_t *words = (const uint32_t *)(blk + (size_t)which * kBlock * HDP);
+  const float scale = ((const float *)(blk + (size_t)2 * kBlock * HDP))[which];
+  const int lo = p.row0 - b * kBlock, hi = lo + p.rows;  // rows lo..hi-1 of the block are asked for
+  const long long ld = (long long)p.H * HD;
+  float *out = (which ? p.values : p.keys) + ((long long)s * p.rows + (long long)b * kBlock - p.row0) * ld + h * HD;
+  auto put = [&](int r, int d, const float4 &x) {
+    if (r < lo || r >= hi || d >= HD) return;
+    float *o = out + r * ld + d;
+    if (HD % 4 == 0) {
+      __stcs((float4 *)o, x);
+    } else {
+      o[0] = x.x;
+      if (d + 1 < HD) o[1] = x.y;
+      if (d + 2 < HD) o[2] = x.z;
+      if (d + 3 < HD) o[3] = x.w;
+    }
+  };
+  if (which == 0) {
+#pragma unroll
+    for (int k = 0; k < HDP / 16; k++) {
+      const int i = threadIdx.x + k * kThreads, r = i / N4, d = (i - r * N4) * 4;
+      const int lane = ((r >> 3) * 2 + (r & 1)) * 4 + ((d & 15) >> 2), wi = ((r & 7) >> 1) * (HDP / 16) + (d >> 4);
+      put(r, d, values4(words[(wi >> 2) * 128 + lane * 4 + (wi & 3)], scale));
+    }
+  } else {
+    for (int i = threadIdx.x; i < 2 * HDP; i += kThreads) {
+      const int r = i / N4 * 4, d = (i - i / N4 * N4) * 4;
+      float4 v[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const int ch = d + c, lane = (ch & 7) * 4 + (r >> 3), wi = (ch >> 3) * 2 + ((r & 7) >> 2);
+        v[c] = values4(words[(wi >> 2) * 128 + lane * 4 + (wi & 3)], scale);
+      }
+      put(r, d, make_float4(v[0].x, v[1].x, v[2].x, v[3].x));
+      put(r + 1, d, make_float4(v[0].y, v[1].y, v[2].y, v[3].y));
+      put(r + 2, d, make_float4(v[0].z, v[1].z, v[2].z, v[3].z));
+      put(r + 3, d, make_float4(v[0].w, v[1].w, v[2].w, v[3].w));
+    }
   }
 }
 
@@ -237,19 +355,19 @@ int fa_kv8_write_rows(fa_ctx *ctx, fa_kv8 *c, const void *k, const void *v, bool
                       const float *counts) {
   if (T == 0) return FA_OK;
   WriteParams p{};
-  p.src[0] = k, p.src[1] = v, p.ld = ld;
+  p.keys = k, p.values = v, p.ld = ld;
   p.codes = c->codes, p.tail = c->tail, p.tag = c->tag;
   p.rows = kv8::Rows{pos, counts, n, T, c->P};
-  p.H = c->H, p.HD = c->HD, p.HDP = c->HDP, p.nblk = c->nblk;
+  p.H = c->H, p.HD = c->HD, p.nblk = c->nblk;
   const uintptr_t mask = f16 ? 7 : 15;
   p.vec = c->HD % 4 == 0 && ld % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & mask) == 0;
   p.status = ctx->dev_status;
   const int touched = pos ? ceil_div(T + kBlock - 1, kBlock) : (n + T - 1) / kBlock - n / kBlock + 1;
   const dim3 grid(touched > 1 ? touched - 1 : 1, 2 * c->H, c->S);  // (the first thread block takes two)
-  const size_t smem = (size_t)kBlock * (c->HDP + 1) * 4;
   {
     LaunchScope ls(ctx, "kv8_write");
-    fa_launch_dep(ctx, f16 ? k_kv8_write<__half> : k_kv8_write<float>, grid, dim3(kThreads), smem, p);
+    if (f16) launch_write<__half>(ctx, p, grid, c->HDP);
+    else launch_write<float>(ctx, p, grid, c->HDP);
   }
   FA_LAUNCH_CHECK(ctx, "kv8_write");
   return FA_OK;
@@ -295,11 +413,13 @@ extern "C" int fa_kv8_read(fa_ctx *ctx, fa_kv8 *c, int row0, int rows, fa_tensor
   int rc = fa_tensor_new(ctx, c->S * rows, c->H * c->HD, FA_F32, true, &v);
   if (rc == FA_OK && rows) {
     ReadParams p{};
-    p.codes = c->codes, p.out[0] = (float *)k->dptr, p.out[1] = (float *)v->dptr;
-    p.row0 = row0, p.rows = rows, p.H = c->H, p.HD = c->HD, p.HDP = c->HDP, p.nblk = c->nblk;
+    p.codes = c->codes, p.keys = (float *)k->dptr, p.values = (float *)v->dptr;
+    p.row0 = row0, p.rows = rows, p.H = c->H, p.HD = c->HD, p.nblk = c->nblk;
     const dim3 grid((row0 + rows - 1) / kBlock - row0 / kBlock + 1, 2 * c->H, c->S);
     LaunchScope ls(ctx, "kv8_read");
-    const cudaError_t e = fa_launch_dep(ctx, k_kv8_read, grid, dim3(kThreads), (size_t)kBlock * c->HDP, p);
+    auto kernel = c->HDP == 32 ? k_kv8_read<32> : c->HDP == 64 ? k_kv8_read<64> : c->HDP == 96 ? k_kv8_read<96>
+                : c->HDP == 128 ? k_kv8_read<128> : k_kv8_read<256>;
+    const cudaError_t e = fa_launch_dep(ctx, kernel, grid, dim3(kThreads), 0, p);
     if (e != cudaSuccess) rc = fa_fail(ctx, FA_ERR_CUDA, "launch kv8_read: %s", cudaGetErrorString(e));
   }
   if (rc != FA_OK) {

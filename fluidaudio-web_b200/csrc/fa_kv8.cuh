@@ -28,25 +28,6 @@ constexpr int kBlock = 32;
 inline int stored_width(int HD) { return HD <= 32 ? 32 : HD <= 64 ? 64 : HD <= 96 ? 96 : HD <= 128 ? 128 : 256; }
 __host__ __device__ constexpr size_t block_bytes(int HDP) { return (size_t)2 * kBlock * HDP + 16; }
 
-// The (position, channel) whose code is byte e of word wi of `lane` in the K or V half of a block.
-__device__ __forceinline__ void k_place(int wi, int lane, int KS, int &pos, int &ch) {
-  const int g = lane >> 2, t = lane & 3, j = wi / KS, ks = wi - j * KS;
-  pos = 8 * (g >> 1) + 2 * j + (g & 1), ch = 16 * ks + 4 * t;  // channels ch..ch+3
-}
-__device__ __forceinline__ void v_place(int wi, int lane, int &pos, int &ch) {
-  const int g = lane >> 2, t = lane & 3;
-  pos = 8 * t + 4 * (wi & 1), ch = 8 * (wi >> 1) + g;  // positions pos..pos+3
-}
-
-__device__ __forceinline__ uint32_t pack4(const int (&q)[4]) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const uint32_t sign = q[e] < 0, mag = (uint32_t)abs(q[e]);
-    w |= e < 2 ? (mag | sign << 15) << (16 * e) : (mag << 8 | sign << 7) << (16 * (e - 2));
-  }
-  return w;
-}
 // code e of a word
 __device__ __forceinline__ float unpack(uint32_t w, int e) {
   const uint32_t half = w >> (16 * (e & 1)), mag = half >> (e < 2 ? 0 : 8) & 0x7f, sign = half >> (e < 2 ? 15 : 7) & 1;
