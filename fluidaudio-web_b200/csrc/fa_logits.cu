@@ -8,14 +8,18 @@
 // and, for a pick, the first token of the largest value among the allowed ones ({-1, -inf} where none is allowed or all are NaN).
 // The reference scans a downloaded row on the host (src/engines/asr-whisper/index.ts:80-97).
 //
-// One pass: a cluster of thread blocks shares a row, each block counts the history's tokens that fall into its slice of the
-// vocabulary in shared memory (whole numbers: the order of the atomics does not show) and then reads its slice of the logits
-// once.  Every operation is rounded by itself, so the values are those of the formulas in f32 whatever the split.
+// One pass: a cluster of thread blocks shares a row.  Each reads its part of the history once and adds to the counters of the
+// block whose slice of the vocabulary a token falls into, in that block's shared memory (whole numbers: the order of the
+// additions does not show), then takes its slice of the logits, whose first loads are under way meanwhile.  Every operation
+// is rounded by itself, so the values are those of the formulas in f32 whatever the split.
+// Bound by HBM where rows are many (4 bytes in, 4 out; the counters stay on the chip), by the latency of two cluster barriers
+// and one round of loads where they are few.
 #include "fa_internal.cuh"
 
 namespace {
 
-constexpr int kThreads = 512, kMaxCluster = 8, kSlice = 16384;  // tokens that a thread block counts at a time (32 KB)
+constexpr int kThreads = 512, kMaxCluster = 8, kBatch = 4;
+constexpr int kSlice = 49152;  // tokens that a thread block counts at a time: 192 KB
 
 struct LogitParams {
   const float *x;
@@ -47,8 +51,21 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <bool PICK>
-__global__ void __launch_bounds__(kThreads) k_adjust(const LogitParams p) {
+__device__ __forceinline__ uint32_t in_block(const void *p, uint32_t rank) {  // the same shared variable in block `rank` of the cluster
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return a;
+}
+
+// n floats from p on into L2, but for what lies outside whole 16-byte groups.
+__device__ __forceinline__ void to_l2(const float *p, int n) {
+  const uintptr_t from = ((uintptr_t)p + 15) & ~(uintptr_t)15, to = (uintptr_t)(p + n) & ~(uintptr_t)15;
+  if (n > 0 && to > from) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from)) : "memory");
+}
+
+// PICK: the best token instead of the logits; HISTORY, BIAS, MASK: which rules there are
+template <bool PICK, bool HISTORY, bool BIAS, bool MASK>
+__global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
   extern __shared__ uint32_t cnt[];  // one slice's counts
   __shared__ float bv[kThreads / 32];
   __shared__ int bi[kThreads / 32];
@@ -57,9 +74,9 @@ __global__ void __launch_bounds__(kThreads) k_adjust(const LogitParams p) {
   fa_grid_dep_sync();
   const int nc = (int)cluster_size(), rank = (int)cluster_rank(), s = blockIdx.x / nc;
   const float *row = p.x + (long long)s * p.ld;
-  const float *bias = p.bias ? p.bias + (p.bias_rows > 1 ? (long long)s * p.bias_ld : 0) : nullptr;
+  const float *bias = BIAS ? p.bias + (p.bias_rows > 1 ? (long long)s * p.bias_ld : 0) : nullptr;
   const uint32_t *mask = nullptr;
-  if (p.mask) {
+  if (MASK) {
     int r = p.mask_rows > 1 ? s : 0;
     if (p.mask_row) {
       const float f = p.mask_row[s];
@@ -71,68 +88,115 @@ __global__ void __launch_bounds__(kThreads) k_adjust(const LogitParams p) {
   }
   float best = -INFINITY;
   int at = 0x7fffffff;
-  const int width = ((p.V + nc - 1) / nc + 31) / 32 * 32, v0 = min(p.V, rank * width), v1 = min(p.V, v0 + width);
-  for (int a = v0; a < v1; a += kSlice) {
-    const int b = min(v1, a + kSlice);
-    if (p.history) {
-      for (int i = threadIdx.x; i < b - a; i += kThreads) cnt[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < p.n; i += kThreads) {
-        const float f = p.history[(long long)i * p.S + s];
-        if (f >= (float)a && f < (float)b) atomicAdd(&cnt[(int)f - a], 1u);
-      }
-      __syncthreads();
+  const int width = ((p.V + nc - 1) / nc + 31) / 32 * 32, v1 = min(p.V, (rank + 1) * width);
+  for (int off = 0; off < width; off += kSlice) {  // (every block of the cluster: they count for one another)
+    const int a = min(p.V, rank * width + off), b = min(v1, a + kSlice);
+    // a thread takes j0, j0 + kThreads, ...: a warp's 32 neighbours share a word of the mask, each its lane's bit
+    const float *px = row + a + threadIdx.x, *pb = BIAS ? bias + a + threadIdx.x : nullptr;
+    const uint32_t *pm = MASK ? mask + ((a + (int)threadIdx.x) >> 5) : nullptr;
+    float *po = PICK ? nullptr : p.out + (long long)s * p.V + a + threadIdx.x;
+    float x[kBatch], bb[BIAS ? kBatch : 1];
+    uint32_t w[MASK ? kBatch : 1];
+    if (threadIdx.x == 0) {  // the slice on its way to L2 while the history is counted
+      to_l2(row + a, b - a);
+      if (BIAS) to_l2(bias + a, b - a);
     }
-    for (int j = a + threadIdx.x; j < b; j += kThreads) {
-      float x = row[j];
-      if (p.history) {
-        const uint32_t c = cnt[j - a];
-        if (c) {
-          x = x > 0.0f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
-          x = __fsub_rn(__fsub_rn(x, __fmul_rn((float)c, p.frequency)), p.presence);
+    int left = b - a - (int)threadIdx.x, k = threadIdx.x;  // tokens from this thread's on, place in the slice
+    auto load = [&]() {
+      if (left > (kBatch - 1) * kThreads) {
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+          x[u] = __ldcs(px + u * kThreads);
+          if (BIAS) bb[u] = __ldcs(pb + u * kThreads);
+          if (MASK) w[u] = pm[u * (kThreads / 32)];
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+          const bool in = u * kThreads < left;
+          x[u] = in ? __ldcs(px + u * kThreads) : 0.0f;
+          if (BIAS) bb[u] = in ? pb[u * kThreads] : 0.0f;
+          if (MASK) w[u] = in ? pm[u * (kThreads / 32)] : 0u;
         }
       }
-      if (bias) x = __fadd_rn(x, bias[j]);
-      const bool allowed = !mask || (mask[j >> 5] >> (j & 31) & 1u);
-      if (PICK) {
-        if (allowed && (x > best || (x == best && j < at))) best = x, at = j;  // (a NaN never wins)
-      } else {
-        p.out[(long long)s * p.V + j] = allowed ? x : -INFINITY;
+      px += kBatch * kThreads;
+      if (BIAS) pb += kBatch * kThreads;
+      if (MASK) pm += kBatch * (kThreads / 32);
+    };
+    load();
+    if (HISTORY) {
+      for (int i = threadIdx.x; i < min(width, kSlice); i += kThreads) cnt[i] = 0;
+      cluster_sync();
+      const int i0 = (int)((long long)p.n * rank / nc), i1 = (int)((long long)p.n * (rank + 1) / nc);
+      for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {
+        const float f = p.history[(long long)i * p.S + s];
+        if (!(f >= 0.0f && f < (float)p.V)) continue;
+        const int token = (int)f, owner = token / width, c = token - owner * width - off;
+        if (c >= 0 && c < kSlice)
+          asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], 1;" ::"r"(in_block(cnt + c, owner)) : "memory");
       }
+      cluster_sync();
     }
-    __syncthreads();
+    auto step = [&](int u) {
+      float y = x[u];
+      if (HISTORY) {
+        const uint32_t c = cnt[k + u * kThreads];
+        if (c) {
+          y = y > 0.0f ? __fdiv_rn(y, p.repetition) : __fmul_rn(y, p.repetition);
+          y = __fsub_rn(__fsub_rn(y, __fmul_rn((float)c, p.frequency)), p.presence);
+        }
+      }
+      if (BIAS) y = __fadd_rn(y, bb[u]);
+      const bool allowed = !MASK || (w[u] >> (threadIdx.x & 31) & 1u);
+      if (PICK) {
+        if (allowed && (y > best || (y == best && a + k + u * kThreads < at))) best = y, at = a + k + u * kThreads;  // (a NaN never wins)
+      } else {
+        __stcs(po + u * kThreads, allowed ? y : -INFINITY);
+      }
+    };
+    while (left > 0) {
+#pragma unroll
+      for (int u = 0; u < kBatch; u++)
+        if (u * kThreads < left) step(u);
+      left -= kBatch * kThreads, k += kBatch * kThreads;
+      if (!PICK) po += kBatch * kThreads;
+      if (left > 0) load();
+    }
+    if (HISTORY && off + kSlice < width) cluster_sync();  // (the counts are read)
   }
   if (!PICK) return;
   auto take = [&](float v, int j) {
     if (v > best || (v == best && j < at)) best = v, at = j;
   };
+  auto warp_best = [&]() {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float v = __shfl_xor_sync(0xffffffffu, best, o);
-    take(v, __shfl_xor_sync(0xffffffffu, at, o));
-  }
+    for (int o = 16; o > 0; o >>= 1) {
+      const float v = __shfl_xor_sync(0xffffffffu, best, o);
+      take(v, __shfl_xor_sync(0xffffffffu, at, o));
+    }
+  };
+  warp_best();
   if ((threadIdx.x & 31) == 0) bv[threadIdx.x >> 5] = best, bi[threadIdx.x >> 5] = at;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; w++) take(bv[w], bi[w]);
-    cv = best, ci = at;
+  if (threadIdx.x < 32) {
+    best = bv[threadIdx.x & (kThreads / 32 - 1)], at = bi[threadIdx.x & (kThreads / 32 - 1)];
+    warp_best();
+    if (threadIdx.x == 0) cv = best, ci = at;
   }
-  cluster_sync();
-  if (rank == 0 && threadIdx.x == 0) {
-    for (int r = 1; r < nc; r++) {
-      float v;
-      int j;
-      uint32_t addr_v, addr_j;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr_v) : "r"((uint32_t)__cvta_generic_to_shared(&cv)), "r"(r));
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr_j) : "r"((uint32_t)__cvta_generic_to_shared(&ci)), "r"(r));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr_v) : "memory");
-      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(j) : "r"(addr_j) : "memory");
-      take(v, j);
+  if (nc > 1) {
+    cluster_sync();
+    if (rank == 0 && threadIdx.x < 32) {
+      const uint32_t r = threadIdx.x & (nc - 1);
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(best) : "r"(in_block(&cv, r)) : "memory");
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(at) : "r"(in_block(&ci, r)) : "memory");
+      warp_best();
     }
+  }
+  if (rank == 0 && threadIdx.x == 0) {
     p.out[2 * s] = at == 0x7fffffff ? -1.0f : (float)at;
     p.out[2 * s + 1] = best;
   }
-  cluster_sync();  // no block leaves while its result is read
+  if (nc > 1) cluster_sync();  // no block leaves while its result is read
 }
 
 int rules(fa_ctx *ctx, const fa_tensor *x, int ncols, const fa_logit_rules *r, bool pick, fa_tensor **out) {
@@ -186,12 +250,19 @@ int rules(fa_ctx *ctx, const fa_tensor *x, int ncols, const fa_logit_rules *r, b
   if (p.S) {
     p.out = (float *)y->dptr, p.status = ctx->dev_status;
     int nc = 1;
-    while (nc < kMaxCluster && (long long)p.S * nc < 2 * ctx->sm_count && p.V > nc * 2048) nc *= 2;
+    while (nc < kMaxCluster && p.V > nc * 2048 && (p.S * nc * 2 <= 3 * ctx->sm_count || p.V > nc * 16640)) nc *= 2;
     const int width = (int)round_up(ceil_div(p.V, nc), 32);
     const size_t smem = p.history ? (size_t)4 * (width < kSlice ? width : kSlice) : 0;
-    static SmemLimit limit[2];
-    auto kernel = pick ? k_adjust<true> : k_adjust<false>;
-    cudaError_t e = limit[pick].raise(ctx, kernel, kSlice * 4);
+    using Kernel = void (*)(LogitParams);
+    static const Kernel kernels[2][8] = {
+        {k_adjust<false, false, false, false>, k_adjust<false, false, false, true>, k_adjust<false, false, true, false>, k_adjust<false, false, true, true>,
+         k_adjust<false, true, false, false>, k_adjust<false, true, false, true>, k_adjust<false, true, true, false>, k_adjust<false, true, true, true>},
+        {k_adjust<true, false, false, false>, k_adjust<true, false, false, true>, k_adjust<true, false, true, false>, k_adjust<true, false, true, true>,
+         k_adjust<true, true, false, false>, k_adjust<true, true, false, true>, k_adjust<true, true, true, false>, k_adjust<true, true, true, true>}};
+    static SmemLimit limit[2][8];
+    const int which = (p.history ? 4 : 0) + (p.bias ? 2 : 0) + (p.mask ? 1 : 0);
+    const Kernel kernel = kernels[pick][which];
+    cudaError_t e = p.history ? limit[pick][which].raise(ctx, kernel, kSlice * 4) : cudaSuccess;
     if (e == cudaSuccess) {
       LaunchScope ls(ctx, pick ? "pick_adjusted" : "adjust_logits");
       cudaLaunchConfig_t cfg{};
