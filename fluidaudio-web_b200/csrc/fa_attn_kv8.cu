@@ -748,9 +748,492 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
   return rc;
 }
 
+// ---- many rows: prompts, or many query heads to a key head ---------------------------------------------------------------
+//
+// 128 rows of a unit against 128 positions at a time on tcgen05: S = Q K^T and O += P V with the accumulators in TMEM, a row to
+// a lane.  Thread block: four warps that hold a row per thread (queries to shared memory, softmax, result), four that turn a
+// cache block each into the f16 tiles of K (position by channel) and V^T (channel by position) in the swizzled K-major layout
+// that the tensor cores read, and one that issues the products.  Both products run twice, with the value and the residue of
+// the rows' side.  P takes the place of S in TMEM, 32 positions at a time (16 columns of values, 16 of residues), and is the
+// TMEM operand of the second product.
+//
+// Weights are exp2(s - ref) times the block's values' scale over the largest scale of the range, times 2^kUpP: whole f16 range
+// for what counts, and the accumulator needs no scale of its own per block.  `ref` is a row's maximum when it was last moved:
+// it moves, and the accumulator is rescaled, only when a tile's maximum is more than 2^kSlack above it.
+//
+// What bounds it: the softmax warps (about 6 instructions an element and one exponential, 16 a clock and SM) and the products,
+// 2 x 128 x 128 x HD x 2 x 2 a tile, cost about the same; two thread blocks an SM overlap them where shared memory allows.
+constexpr int kPromptRows = 49;  // from here on
+constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6, kSlack = 8;
+
+template <int HDP>
+struct PromptSmem {
+  static constexpr int CH = (HDP + 63) / 64;                                      // 64-channel chunks of a row
+  static constexpr int Q = 0, K = Q + 2 * CH * 16384, V = K + CH * 16384, STAGE = V + 2 * HDP * 128;
+  static constexpr int STAGE_BYTES = (4 * (int)kv8::block_bytes(HDP) + 127) / 128 * 128, BYTES = STAGE + 2 * STAGE_BYTES + 1024;
+};
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t a[16], b[16];
+  tc::tmem_ld16(addr, a);
+  tc::tmem_ld16(addr + 16, b);
+  tc::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(a[i]), v[16 + i] = __uint_as_float(b[i]);
+}
+// D (+)= A B with A in TMEM (16 f16 of a row in 8 columns) and B in shared memory
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct PromptParams {
+  AttnParams a;
+  int rowtiles, splits, per;  // row tiles of a unit, splits of the positions and their tiles
+};
+
+template <int HDP>
+__global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv8(const PromptParams pp) {
+  using Smem = PromptSmem<HDP>;
+  constexpr int KS = HDP / 16, CH = Smem::CH, BB = (int)kv8::block_bytes(HDP), kWaits = 81, kColumns = HDP <= 64 ? 256 : 512;
+  const AttnParams &p = pp.a;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
+  __shared__ __align__(8) uint64_t bar[8];  // see the names below
+  __shared__ float scl[2][4][2];            // a tile's scales: keys; values over the largest
+  __shared__ float svmax_of[kPromptThreads / 32];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up;
+  const uint32_t s_full = smem_u32(&bar[0]), p_full = smem_u32(&bar[1]), pv_done = smem_u32(&bar[2]), k_full = smem_u32(&bar[3]),
+                 v_full = smem_u32(&bar[4]), code_free = smem_u32(&bar[5]), code_full = smem_u32(&bar[6]);  // (two stages)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  int at = blockIdx.x;
+  const int split = at % pp.splits;
+  at /= pp.splits;
+  const int rt = pp.rowtiles - 1 - at % pp.rowtiles, unit = at / pp.rowtiles, s = unit / p.H, h = unit - s * p.H;  // (longest first)
+  if (tid == 0) {
+    tc::mbar_init(s_full, 2);  // the products, and who issued them: the scales of the tile come with it
+    tc::mbar_init(p_full, kTile);
+    tc::mbar_init(pv_done, 1);
+    tc::mbar_init(k_full, 128);
+    tc::mbar_init(v_full, 128);
+    tc::mbar_init(code_free, 128);
+    tc::mbar_init(code_full, 1);
+    tc::mbar_init(code_full + 8, 1);
+    tc::fence_barrier_init();
+    gave_up = 0;
+  }
+  if (warp == 8) tc::tmem_alloc(smem_u32(&tmem_slot), kColumns);
+  __syncthreads();  // in front of the next grid's start, which may want columns too
+  fa_grid_dep_sync();
+
+  Sight sight;
+  bool bad;
+  sight.of(p, s, bad);
+  if (bad && tid == 0) atomicOr(p.status + 3, kStatusKv8Length);
+  const int nrows = p.G * p.T, row_a = rt * kTile, row_b = min(nrows, row_a + kTile) - 1;
+  int most = sight.len;
+  if (p.causal) {
+    const int i = min(row_b / p.G, sight.count - 1);
+    most = i >= row_a / p.G ? sight.start + i + 1 : 0;
+  }
+  const int t0 = split * pp.per, t1 = min((most + kTile - 1) / kTile, t0 + pp.per), nt = max(0, t1 - t0);
+  const uint8_t *codes = p.codes + (size_t)unit * p.nblk * BB;
+
+  // the largest scale of the range's values
+  float svmax = 0.0f;
+  for (int b = t0 * 4 + tid; b < min(t1 * 4, (most + kBlock - 1) / kBlock); b += kPromptThreads) {
+    const float sv = *(const float *)(codes + (size_t)b * BB + 2 * kBlock * HDP + 4);
+    if (sv < INFINITY) svmax = fmaxf(svmax, sv);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) svmax = fmaxf(svmax, __shfl_xor_sync(0xffffffffu, svmax, o));
+  if (lane == 0) svmax_of[warp] = svmax;
+
+  // queries: this thread's row, scaled and split as in load_row
+  const int row = row_a + tid;
+  float qs = 0.0f;
+  if (warp < 4) {
+    const int rr = min(row, nrows - 1), i = rr / p.G;
+    const float *qp = p.q + ((long long)s * p.T + i) * p.ldq + (h * p.G + rr - i * p.G) * p.HD;
+    auto four = [&](int d) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < nrows && d < p.HD) {
+        if (p.vec) {
+          v = *(const float4 *)(qp + d);
+        } else {
+          v.x = qp[d];
+          if (d + 1 < p.HD) v.y = qp[d + 1];
+          if (d + 2 < p.HD) v.z = qp[d + 2];
+          if (d + 3 < p.HD) v.w = qp[d + 3];
+        }
+      }
+      return v;
+    };
+    uint32_t a = 0;
+#pragma unroll 4
+    for (int d = 0; d < HDP; d += 4) {
+      const float4 v = four(d);
+      a = max(max(a, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu)),
+              max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+    }
+    const int bits = (int)(a >> 23), ex = min(max(bits, kUp + 1), 254);
+    const float f = __int_as_float((254 + kUp - ex) << 23);
+    qs = bits < 255 ? __int_as_float(ex << 23) : __int_as_float(0x7fc00000);
+#pragma unroll 2
+    for (int u = 0; u < HDP / 8; u++) {  // 16 bytes: eight channels
+      const float4 x = four(8 * u), y = four(8 * u + 4);
+      uint32_t hi[4], lo[4];
+      split2(x.x * f, x.y * f, hi[0], lo[0]);
+      split2(x.z * f, x.w * f, hi[1], lo[1]);
+      split2(y.x * f, y.y * f, hi[2], lo[2]);
+      split2(y.z * f, y.w * f, hi[3], lo[3]);
+      uint8_t *dst = smem + Smem::Q + (u >> 3) * 16384 + tid * 128 + (((u & 7) ^ (tid & 7)) << 4);
+      *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *(uint4 *)(dst + CH * 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    tc::fence_proxy_async_smem();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_slot, tS = tmem, tO = tmem + 128, tSum = tO + HDP;
+  svmax = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kPromptThreads / 32; w++) svmax = fmaxf(svmax, svmax_of[w]);
+  if (!(svmax > 0.0f)) svmax = 1.0f;
+  auto wait = [&](uint32_t b, uint32_t parity) { return tc::mbar_wait(b, parity, p.wait_limit); };
+  bool ok = true;
+  float m = -INFINITY, l = 0.0f;
+
+  if (warp < 4) {  // ---- a row per thread
+    const int lim = row < nrows ? sight.limit(row / p.G) : 0;
+    const uint32_t mine = (uint32_t)(warp * 32) << 16;
+    // what the tile before gave joins the running result, and both go to the new reference: the tensor cores cut off what an f32
+    // cannot hold, so a sum that ran on over many tiles would shrink; within a tile the residues go first
+    auto sum_up = [&](bool more, float f) {
+#pragma unroll 1
+      for (int c = 0; c < HDP; c += 16) {
+        uint32_t x[16], y[16];
+        tc::tmem_ld16(tO + mine + c, x);
+        if (more) tc::tmem_ld16(tSum + mine + c, y);
+        tc::tmem_ld_wait();
+        if (more) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(x[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+        tmem_st16(tSum + mine + c, x);
+      }
+    };
+    for (int k = 0; k < nt && ok; k++) {
+      ok = wait(s_full, k & 1);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc::tc_fence_after();
+      const int first = (t0 + k) * kTile;
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) {
+        float v[32];
+        tmem_ld32(tS + mine + 32 * c, v);
+        const int n = lim - first - 32 * c;
+        float t = -INFINITY;
+        if (__all_sync(0xffffffffu, n >= 32)) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) t = fmaxf(t, v[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) t = e < n ? fmaxf(t, v[e]) : t;
+        }
+        if (n > 0) top = fmaxf(top, t * (scl[k & 1][c][0] * kScoreUnit * qs));
+      }
+      // a new reference where the maximum has moved far: what was summed so far is rescaled
+      const bool move = top > m + kSlack || (m == -INFINITY && top > -INFINITY);
+      const float old = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+      if (move) m = top, l *= old;
+      if (k > 0) sum_up(k > 1, old);
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) {
+        float v[32];
+        tmem_ld32(tS + mine + 32 * c, v);
+        const int n = lim - first - 32 * c;
+        const float f = scl[k & 1][c][0] * kScoreUnit * qs, wf = scl[k & 1][c][1];
+        const bool all = __all_sync(0xffffffffu, n >= 32);
+        uint32_t out[32];
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x = ex2(fmaf(v[e], f, -ref)), y = ex2(fmaf(v[e + 1], f, -ref));
+          if (!all) x = e < n ? x : 0.0f, y = e + 1 < n ? y : 0.0f;
+          sum0 += x, sum1 += y;
+          x *= wf, y *= wf;
+          if (!all) x = e < n ? x : 0.0f, y = e + 1 < n ? y : 0.0f;  // (a masked place's scale may be NaN)
+          split2(x, y, out[e >> 1], out[16 + (e >> 1)]);
+        }
+        l += sum0 + sum1;
+        tmem_st32(tS + mine + 32 * c, out);
+      }
+      tmem_st_wait();
+      tc::tc_fence_before();
+      tc::mbar_arrive(p_full);
+    }
+    if (nt > 0 && __all_sync(0xffffffffu, ok)) ok = wait(pv_done, (nt - 1) & 1);
+    ok = __all_sync(0xffffffffu, ok);
+    tc::tc_fence_after();
+    const bool sees = lim > 0;
+    const int i = row / p.G, C = p.H * p.G * p.HD, col0 = (h * p.G + row - i * p.G) * p.HD;
+    const long long orow = (long long)s * p.T + i;
+    const float unit_of = exp2f(24 - kUpP), inv = pp.splits == 1 ? unit_of / l : unit_of;
+    const size_t part = ((size_t)unit * pp.splits + split) * nrows + row;
+    if (pp.splits > 1 && row < nrows) *(float2 *)(p.pml + part * 2) = make_float2(m, l);
+    for (int c = 0; c < HDP; c += 16) {
+      uint32_t x[16];
+      __syncwarp();
+      if (nt > 0) {
+        uint32_t y[16];
+        tc::tmem_ld16(tO + mine + c, x);
+        if (nt > 1) tc::tmem_ld16(tSum + mine + c, y);
+        tc::tmem_ld_wait();
+        if (nt > 1) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(x[e]));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[e] = nt > 0 && sees ? __float_as_uint(__uint_as_float(x[e]) * inv * svmax) : 0u;
+      float *dst = pp.splits > 1 ? p.pacc + part * HDP + c : p.out + orow * C + col0 + c;
+      if (row < nrows && (pp.splits > 1 || (p.HD % 16 == 0 && c < p.HD))) {  // whole groups of 16 channels, 64 bytes aligned
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *(uint4 *)(dst + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        if (p.y16 && pp.splits == 1) {
+          __half *d16 = p.y16 + ((long long)((col0 + c) >> 6) * p.R + orow) * 64 + ((col0 + c) & 63);
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) split2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]), hi[e], lo[e]);
+          *(uint4 *)d16 = make_uint4(hi[0], hi[1], hi[2], hi[3]), *(uint4 *)(d16 + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+          if (p.lo_off) {
+            *(uint4 *)(d16 + p.lo_off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *(uint4 *)(d16 + p.lo_off + 8) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+          }
+        }
+      } else if (row < nrows && c < p.HD) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          if (c + e < p.HD) {
+            const float y = __uint_as_float(x[e]);
+            dst[e] = y;
+            if (p.y16) {
+              const int col = col0 + c + e;
+              __half *d16 = p.y16 + ((long long)(col >> 6) * p.R + orow) * 64 + (col & 63);
+              const __half hi = __float2half_rn(y);
+              *d16 = hi;
+              if (p.lo_off) d16[p.lo_off] = __float2half_rn(y - __half2float(hi));
+            }
+          }
+        }
+      }
+    }
+    tc::tc_fence_before();
+  } else if (warp < 8) {  // ---- codes to tiles, a cache block per warp
+    const int w = warp - 4;
+    auto fetch = [&](int k) {  // tile k of this range into stage k & 1
+      const int b = (t0 + k) * 4, n = min(4, p.nblk - b);
+      const uint32_t bytes = (uint32_t)n * BB, dst = smem_u32(smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES), on = code_full + 8 * (k & 1);
+      tc::mbar_expect_tx(on, bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(codes + (size_t)b * BB),
+                   "r"(bytes), "r"(on)
+                   : "memory");
+    };
+    int fetched = 0;
+    if (tid == 128)
+      for (; fetched < min(2, nt); fetched++) fetch(fetched);
+    fetched = min(2, nt);
+    int k = 0;
+    for (; k < nt && ok; k++) {
+      ok = wait(code_full + 8 * (k & 1), (k >> 1) & 1);
+      const uint8_t *blk = smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES + w * BB;
+      if (k > 0) ok = ok && wait(s_full, (k - 1) & 1);  // the products of the tile before have read K
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+      for (int c = 0; c < KS; c++) {
+        const uint4 w4 = *(const uint4 *)(blk + c * 512 + lane * 16);
+        const uint32_t word[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int wi = 4 * c + u, j = wi / KS, ks = wi % KS, r = w * 32 + 8 * (g >> 1) + 2 * j + (g & 1), ch = 16 * ks + 4 * t;
+          uint2 x;
+          widen(word[u], x.x, x.y);
+          *(uint2 *)(smem + Smem::K + (ch >> 6) * 16384 + r * 128 + ((((ch & 63) >> 3) ^ (r & 7)) << 4) + (ch & 4) * 2) = x;
+        }
+      }
+      if (lane == 0) {
+        const bool there = (t0 + k) * 4 + w < p.nblk;
+        const float2 sc = there ? *(const float2 *)(blk + 2 * kBlock * HDP) : make_float2(0.f, 0.f);
+        scl[k & 1][w][0] = sc.x, scl[k & 1][w][1] = sc.y / svmax * (float)(1 << kUpP);
+      }
+      tc::fence_proxy_async_smem();
+      tc::mbar_arrive(k_full);
+      if (k > 0) ok = wait(pv_done, (k - 1) & 1);  // and V
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+      for (int c = 0; c < KS; c++) {
+        const uint4 w4 = *(const uint4 *)(blk + kBlock * HDP + c * 512 + lane * 16);
+        uint4 x, y;
+        widen(w4.x, x.x, x.y);
+        widen(w4.y, x.z, x.w);
+        widen(w4.z, y.x, y.y);
+        widen(w4.w, y.z, y.w);
+        const int ch = 16 * c + g, u = 4 * (w & 1) + t;  // channels ch and ch + 8, positions 32 w + 8t ..+7
+        uint8_t *dst = smem + Smem::V + (w >> 1) * (HDP * 128) + ch * 128 + ((u ^ (ch & 7)) << 4);
+        *(uint4 *)dst = x, *(uint4 *)(dst + 1024) = y;
+      }
+      tc::fence_proxy_async_smem();
+      tc::mbar_arrive(v_full);
+      tc::mbar_arrive(code_free);
+      if (fetched < nt) {
+        if (tid == 128 && wait(code_free, k & 1)) fetch(fetched);  // (where this runs out, so does the wait for the tile)
+        fetched++;
+      }
+    }
+    if (!ok) gave_up = 1;
+    for (; k < fetched; k++)  // (only behind a wait that ran out) copies of one's own still under way
+      wait(code_full + 8 * (k & 1), (k >> 1) & 1);
+  } else if (lane == 0) {  // ---- products
+    const uint32_t id_s = tc::make_idesc(0, kTile, kTile), id_o = tc::make_idesc(0, kTile, HDP);
+    const uint32_t q0 = smem_u32(smem + Smem::Q), k0 = smem_u32(smem + Smem::K), v0 = smem_u32(smem + Smem::V);
+    for (int k = 0; k < nt && ok; k++) {
+      ok = wait(k_full, k & 1) && (k == 0 || wait(pv_done, (k - 1) & 1));
+      if (!ok) break;
+      tc::tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < 2; part++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+          const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
+          tc::umma<0>(tS, tc::smem_desc_sw128(q0 + (1 - part) * (CH * 16384) + off), tc::smem_desc_sw128(k0 + off), id_s, part + ks > 0);
+        }
+      tc::umma_commit(s_full);
+      tc::mbar_arrive(s_full);
+      ok = wait(v_full, k & 1) && wait(p_full, k & 1);
+      if (!ok) break;
+      tc::tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < 2; part++)
+#pragma unroll
+        for (int step = 0; step < 8; step++)  // 16 positions
+          umma_ts(tO, tS + (step >> 1) * 32 + (1 - part) * 16 + (step & 1) * 8, tc::smem_desc_sw128(v0 + (step >> 2) * (HDP * 128) + (step & 3) * 32),
+                  id_o, part + step > 0);
+      tc::umma_commit(pv_done);
+    }
+    if (!ok) gave_up = 1;
+  }
+  if (warp < 4 && !ok) gave_up = 1;
+  __syncthreads();
+  if (gave_up && tid == 0) {
+    atomicExch(p.status, kWaits + 1);
+    p.status[1] = blockIdx.x, p.status[2] = 0;
+  }
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, kColumns);
+  }
+}
+
+// Rows of several splits: one warp a row.
+template <int HDP>
+__global__ void __launch_bounds__(kThreads) k_join_kv8(const AttnParams p, int splits, int nrows, long long total) {
+  fa_grid_dep_sync();
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (id >= total) return;
+  const int unit = (int)(id / nrows), row = (int)(id - (long long)unit * nrows), s = unit / p.H, h = unit - s * p.H;
+  Sight sight;
+  bool bad;
+  sight.of(p, s, bad);
+  Joined<HDP> j;
+  for (int k = 0; k < splits; k++) {
+    const size_t part = ((size_t)unit * splits + k) * nrows + row;
+    const float2 ml = *(const float2 *)(p.pml + part * 2);
+    float v[HDP / 32];
+#pragma unroll
+    for (int i = 0; i < HDP / 32; i++) v[i] = p.pacc[part * HDP + lane + 32 * i];
+    j.add(ml.x, ml.y, v);
+  }
+  j.L *= kValueUnit;  // (these parts are in the values' own unit)
+  j.finish(p, s, h, row, sight.limit(row / p.G) > 0, lane);
+}
+
+template <int HDP>
+int run_prompt(fa_ctx *ctx, const fa_kv8 *c, const AttnParams &a, int most, const char *label) {
+  static SmemLimit limit;
+  constexpr int smem = PromptSmem<HDP>::BYTES;
+  FA_CHECK_CUDA(ctx, limit.raise(ctx, k_prompt_kv8<HDP>, smem));
+  PromptParams pp{};
+  pp.a = a;
+  const int nrows = a.G * a.T, tiles = ceil_div(most < 1 ? 1 : most, kTile);
+  pp.rowtiles = ceil_div(nrows, kTile);
+  const long long blocks = (long long)c->S * c->H * pp.rowtiles, slots = (long long)ctx->sm_count * (HDP <= 64 ? 2 : 1);
+  // the positions are split while the thread blocks do not fill the GPU once, four tiles a split at least
+  long long splits = blocks >= slots ? 1 : slots / blocks;
+  if (splits > tiles / 4) splits = tiles / 4;
+  if (splits < 1) splits = 1;
+  pp.per = ceil_div(tiles, (int)splits);
+  pp.splits = ceil_div(tiles, pp.per);
+  FA_REQUIRE(ctx, blocks * pp.splits <= 0x7fffffffLL, "%s: too many rows in one call", label);
+  void *scratch = nullptr;
+  size_t bytes = 0;
+  const long long total = (long long)c->S * c->H * nrows;
+  if (pp.splits > 1) {
+    const size_t n = (size_t)total * pp.splits;
+    FA_TRY(fa_block_acquire(ctx, n * (HDP + 2) * 4, &scratch, &bytes));
+    pp.a.pacc = (float *)scratch, pp.a.pml = (float *)scratch + n * HDP;
+  }
+  int rc = FA_OK;
+  cudaError_t e;
+  {
+    LaunchScope ls(ctx, label);
+    e = fa_launch_dep(ctx, k_prompt_kv8<HDP>, dim3((unsigned)(blocks * pp.splits)), dim3(kPromptThreads), (size_t)smem, pp);
+  }
+  if (e == cudaSuccess && pp.splits > 1) {
+    LaunchScope ls(ctx, "attn_kv8_join");
+    e = fa_launch_dep(ctx, k_join_kv8<HDP>, dim3((unsigned)((total + kWarps - 1) / kWarps)), dim3(kThreads), 0, pp.a, pp.splits, nrows, total);
+  }
+  if (e != cudaSuccess) rc = fa_fail(ctx, FA_ERR_CUDA, "launch %s: %s", label, cudaGetErrorString(e));
+  if (scratch) fa_block_release(ctx, scratch);
+  return rc;
+}
+
 template <int HDP>
 int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label) {
   const int rows = p.G * p.T;
+  if constexpr (HDP <= 128) {
+    if (rows >= kPromptRows) return run_prompt<HDP>(ctx, c, p, most, label);
+  }
   if (rows <= 4) return run<HDP, FewRows<HDP>>(ctx, c, p, most, label);
   if constexpr (HDP <= 128) {  // (16 rows of 256 do not fit the registers)
     if (rows > 8) return run<HDP, ManyRows<HDP, 2>>(ctx, c, p, most, label);
