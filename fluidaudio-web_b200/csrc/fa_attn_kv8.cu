@@ -10,6 +10,8 @@
 #include "fa_kv8.cuh"
 #include "fa_tc_common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 using kv8::kBlock;
@@ -750,12 +752,12 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 
 // ---- many rows: prompts, or many query heads to a key head ---------------------------------------------------------------
 //
-// 128 rows of a unit against 128 positions at a time on tcgen05: S = Q K^T and O += P V with the accumulators in TMEM, a row to
-// a lane.  Thread block: four warps that hold a row per thread (queries to shared memory, softmax, result), four that turn a
-// cache block each into the f16 tiles of K (position by channel) and V^T (channel by position) in the swizzled K-major layout
-// that the tensor cores read, and one that issues the products.  Both products run twice, with the value and the residue of
-// the rows' side.  P takes the place of S in TMEM, 32 positions at a time (16 columns of values, 16 of residues), and is the
-// TMEM operand of the second product.
+// 128 rows of a unit against 128 positions at a time on tcgen05: S = Q K^T and O = P V with the accumulators in TMEM, a row to
+// a lane.  Eight warps, two threads a row with half of the positions each, turn cache blocks into the f16 tiles of K (position
+// by channel) and V^T (channel by position) in the swizzled K-major layout that the tensor cores read, and do the softmax; a
+// ninth issues the products.  Both products run twice, with the value and the residue of the rows' side.  P takes the place of
+// S in TMEM, 32 positions at a time (16 columns of values, 16 of residues), and is the TMEM operand of the second product.
+// The next tile's K is made while a tile's P V runs and its V while its own scores are computed.
 //
 // Weights are exp2(s - ref) times the block's values' scale over the largest scale of the range, times 2^kUpP: whole f16 range
 // for what counts, and the accumulator needs no scale of its own per block.  `ref` is a row's maximum when it was last moved:
@@ -763,7 +765,9 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 //
 // What bounds it: the softmax warps (about 6 instructions an element and one exponential, 16 a clock and SM) and the products,
 // 2 x 128 x 128 x HD x 2 x 2 a tile, cost about the same; two thread blocks an SM overlap them where shared memory allows.
-constexpr int kPromptRows = 49;  // from here on
+// From this many rows of a unit on.  Measured, us, groups of 16 rows / this kernel, 16 streams of 20 heads of 64 over 1500
+// positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.
+constexpr int kPromptRows = 49;
 constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6, kSlack = 8;
 
 template <int HDP>
@@ -799,6 +803,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(a[i]), v[16 + i] = __uint_as_float(b[i]);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // D (+)= A B with A in TMEM (16 f16 of a row in 8 columns) and B in shared memory
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -821,7 +830,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t bar[8];  // see the names below
-  __shared__ float scl[2][4][2];            // a tile's scales: keys; values over the largest
+  __shared__ float tops[2][2][kTile];        // row maxima of the two halves; their sums of weights in the end
+  __shared__ float scl[2][4][4];            // a tile's scales: keys, in units of log 2; values over the largest, log and reciprocal
   __shared__ float svmax_of[kPromptThreads / 32];
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
@@ -835,11 +845,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   const int rt = pp.rowtiles - 1 - at % pp.rowtiles, unit = at / pp.rowtiles, s = unit / p.H, h = unit - s * p.H;  // (longest first)
   if (tid == 0) {
     tc::mbar_init(s_full, 2);  // the products, and who issued them: the scales of the tile come with it
-    tc::mbar_init(p_full, kTile);
+    tc::mbar_init(p_full, 256);
     tc::mbar_init(pv_done, 1);
-    tc::mbar_init(k_full, 128);
-    tc::mbar_init(v_full, 128);
-    tc::mbar_init(code_free, 128);
+    tc::mbar_init(k_full, 256);
+    tc::mbar_init(v_full, 256);
+    tc::mbar_init(code_free, 256);
     tc::mbar_init(code_full, 1);
     tc::mbar_init(code_full + 8, 1);
     tc::fence_barrier_init();
@@ -862,60 +872,78 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   const int t0 = split * pp.per, t1 = min((most + kTile - 1) / kTile, t0 + pp.per), nt = max(0, t1 - t0);
   const uint8_t *codes = p.codes + (size_t)unit * p.nblk * BB;
 
-  // the largest scale of the range's values
-  float svmax = 0.0f;
+  // everything that is read first is asked for together: the codes of two tiles, the query rows, the values' scales
+  auto fetch = [&](int k) {  // tile k of this range into stage k & 1
+    const int b = (t0 + k) * 4, n = min(4, p.nblk - b);
+    const uint32_t bytes = (uint32_t)n * BB, dst = smem_u32(smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES), on = code_full + 8 * (k & 1);
+    tc::mbar_expect_tx(on, bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(codes + (size_t)b * BB),
+                 "r"(bytes), "r"(on)
+                 : "memory");
+  };
+  int fetched = min(2, nt);  // tiles asked for
+  if (tid == 0)
+    for (int k = 0; k < fetched; k++) fetch(k);
+  // a row's channels over LPR lanes
+  constexpr int LPR = HDP <= 32 ? 8 : HDP <= 64 ? 16 : 32, PER = LPR / 2;  // rows of a thread
+  const int sub = tid & (LPR - 1), d0 = sub * 4, line = tid / LPR;
+  auto of_row = [&](int r, int &i, int &head) {  // row of the tile -> query, query head
+    const int rr = min(row_a + r, nrows - 1);
+    i = rr / p.G, head = h * p.G + rr - i * p.G;
+  };
+  float4 x[PER];
+  if (warp < 8) {
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int r = line + k * (256 / LPR);
+      int i, head;
+      of_row(r, i, head);
+      const float *qp = p.q + ((long long)s * p.T + i) * p.ldq + head * p.HD + d0;
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row_a + r < nrows && d0 < p.HD) {
+        if (p.vec) {
+          x[k] = *(const float4 *)qp;
+        } else {
+          x[k].x = qp[0];
+          if (d0 + 1 < p.HD) x[k].y = qp[1];
+          if (d0 + 2 < p.HD) x[k].z = qp[2];
+          if (d0 + 3 < p.HD) x[k].w = qp[3];
+        }
+      }
+    }
+  }
+  float svmax = 0.0f;  // the largest scale of the range's values
   for (int b = t0 * 4 + tid; b < min(t1 * 4, (most + kBlock - 1) / kBlock); b += kPromptThreads) {
     const float sv = *(const float *)(codes + (size_t)b * BB + 2 * kBlock * HDP + 4);
     if (sv < INFINITY) svmax = fmaxf(svmax, sv);
   }
+  // queries scaled and split as in load_row
+  if (warp < 8) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) svmax = fmaxf(svmax, __shfl_xor_sync(0xffffffffu, svmax, o));
-  if (lane == 0) svmax_of[warp] = svmax;
-
-  // queries: this thread's row, scaled and split as in load_row
-  const int row = row_a + tid;
-  float qs = 0.0f;
-  if (warp < 4) {
-    const int rr = min(row, nrows - 1), i = rr / p.G;
-    const float *qp = p.q + ((long long)s * p.T + i) * p.ldq + (h * p.G + rr - i * p.G) * p.HD;
-    auto four = [&](int d) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < nrows && d < p.HD) {
-        if (p.vec) {
-          v = *(const float4 *)(qp + d);
-        } else {
-          v.x = qp[d];
-          if (d + 1 < p.HD) v.y = qp[d + 1];
-          if (d + 2 < p.HD) v.z = qp[d + 2];
-          if (d + 3 < p.HD) v.w = qp[d + 3];
-        }
+    for (int k = 0; k < PER; k++) {
+      const int r = line + k * (256 / LPR);
+      uint32_t a = max(max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu),
+                       max(__float_as_uint(x[k].z) & 0x7fffffffu, __float_as_uint(x[k].w) & 0x7fffffffu));
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+      const int bits = (int)(a >> 23), ex = min(max(bits, kUp + 1), 254);
+      const float f = __int_as_float((254 + kUp - ex) << 23);
+      if (sub == 0) tops[0][0][r] = bits < 255 ? __int_as_float(ex << 23) : __int_as_float(0x7fc00000);
+      if (d0 < HDP) {
+        uint2 hi, lo;
+        split2(x[k].x * f, x[k].y * f, hi.x, lo.x);
+        split2(x[k].z * f, x[k].w * f, hi.y, lo.y);
+        uint8_t *dst = smem + Smem::Q + (d0 >> 6) * 16384 + r * 128 + ((((d0 & 63) >> 3) ^ (r & 7)) << 4) + (d0 & 4) * 2;
+        *(uint2 *)dst = hi;
+        *(uint2 *)(dst + CH * 16384) = lo;
       }
-      return v;
-    };
-    uint32_t a = 0;
-#pragma unroll 4
-    for (int d = 0; d < HDP; d += 4) {
-      const float4 v = four(d);
-      a = max(max(a, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu)),
-              max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
-    }
-    const int bits = (int)(a >> 23), ex = min(max(bits, kUp + 1), 254);
-    const float f = __int_as_float((254 + kUp - ex) << 23);
-    qs = bits < 255 ? __int_as_float(ex << 23) : __int_as_float(0x7fc00000);
-#pragma unroll 2
-    for (int u = 0; u < HDP / 8; u++) {  // 16 bytes: eight channels
-      const float4 x = four(8 * u), y = four(8 * u + 4);
-      uint32_t hi[4], lo[4];
-      split2(x.x * f, x.y * f, hi[0], lo[0]);
-      split2(x.z * f, x.w * f, hi[1], lo[1]);
-      split2(y.x * f, y.y * f, hi[2], lo[2]);
-      split2(y.z * f, y.w * f, hi[3], lo[3]);
-      uint8_t *dst = smem + Smem::Q + (u >> 3) * 16384 + tid * 128 + (((u & 7) ^ (tid & 7)) << 4);
-      *(uint4 *)dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *(uint4 *)(dst + CH * 16384) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     tc::fence_proxy_async_smem();
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) svmax = fmaxf(svmax, __shfl_xor_sync(0xffffffffu, svmax, o));
+  if (lane == 0) svmax_of[warp] = svmax;
+  const int quad = warp & 3, half = warp >> 2, local = quad * 32 + lane, row = row_a + local;
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -924,52 +952,125 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
 #pragma unroll
   for (int w = 0; w < kPromptThreads / 32; w++) svmax = fmaxf(svmax, svmax_of[w]);
   if (!(svmax > 0.0f)) svmax = 1.0f;
-  auto wait = [&](uint32_t b, uint32_t parity) { return tc::mbar_wait(b, parity, p.wait_limit); };
+  const float qs = tops[0][0][local];
+  __syncthreads();  // (the array's next use)
+  // Where a wait runs out a thread goes on without waiting for anything: every loop ends, every barrier gets its arrivals, and
+  // the status word makes the result void.
   bool ok = true;
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (ok) ok = tc::mbar_wait(b, parity, p.wait_limit);
+  };
   float m = -INFINITY, l = 0.0f;
 
-  if (warp < 4) {  // ---- a row per thread
+  if (warp < 8) {
+    const int g = lane >> 2, t = lane & 3;
+    // a warp's share of tile k: block `quad`, half of its channels
+    auto stage = [&](int k) { return smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES + quad * BB; };
+    auto keys = [&](int k) {
+      wait(code_full + 8 * (k & 1), (k >> 1) & 1);
+      __syncwarp();
+      const uint8_t *blk = stage(k);
+      // position r = 32 quad + 8 (g/2) + 2j + g%2, 16-byte unit 2 (ks%4) + t/2 of its row: swizzled, 2 (ks%4 ^ j) + (t/2 ^ g%2)
+      uint8_t *dst = smem + Smem::K + (quad * 32 + 8 * (g >> 1) + (g & 1)) * 128 + (((t >> 1) ^ (g & 1)) << 4) + (t & 1) * 8;
+      auto part = [&](auto which) {
+        constexpr int kHalf = decltype(which)::value;
+#pragma unroll
+        for (int c = kHalf * (KS / 2); c < (kHalf + 1) * (KS / 2); c++) {
+          const uint4 w4 = *(const uint4 *)(blk + c * 512 + lane * 16);
+          const uint32_t word[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const int j = (4 * c + u) / KS, ks = (4 * c + u) % KS;
+            uint2 x;
+            widen(word[u], x.x, x.y);
+            *(uint2 *)(dst + (ks >> 2) * 16384 + j * 256 + (((ks & 3) ^ j) << 5)) = x;
+          }
+        }
+      };
+      if (half == 0) part(std::integral_constant<int, 0>());
+      else part(std::integral_constant<int, 1>());
+      if (half == 0 && lane == 0) {
+        const bool there = (t0 + k) * 4 + quad < p.nblk;
+        const float2 sc = there ? *(const float2 *)(blk + 2 * kBlock * HDP) : make_float2(0.f, 0.f);
+        // a scale of 0 stands with codes of 0, one of 2^-60 of the largest counts for nothing: both may be any other
+        const float v = sc.y / svmax;
+        const float wf = (v < 8.7e-19f ? 8.7e-19f : v) * (float)(1 << kUpP);
+        scl[k & 1][quad][0] = sc.x * kScoreUnit, scl[k & 1][quad][1] = __log2f(wf), scl[k & 1][quad][2] = 1.0f / wf;
+      }
+      tc::fence_proxy_async_smem();
+      tc::mbar_arrive(k_full);
+    };
+    auto values = [&](int k) {
+      const uint8_t *blk = stage(k) + kBlock * HDP;
+#pragma unroll
+      for (int cc = 0; cc < KS / 2; cc++) {
+        const int c = half * (KS / 2) + cc;
+        const uint4 w4 = *(const uint4 *)(blk + c * 512 + lane * 16);
+        uint4 x, y;
+        widen(w4.x, x.x, x.y);
+        widen(w4.y, x.z, x.w);
+        widen(w4.z, y.x, y.y);
+        widen(w4.w, y.z, y.w);
+        const int ch = 16 * c + g, u = 4 * (quad & 1) + t;  // channels ch and ch + 8, positions 32 quad + 8t ..+7
+        uint8_t *dst = smem + Smem::V + (quad >> 1) * (HDP * 128) + ch * 128 + ((u ^ (ch & 7)) << 4);
+        *(uint4 *)dst = x, *(uint4 *)(dst + 1024) = y;
+      }
+      tc::fence_proxy_async_smem();
+      tc::mbar_arrive(v_full);
+      tc::mbar_arrive(code_free);
+      if (fetched < nt) {
+        if (tid == 0) wait(code_free, k & 1), fetch(fetched);
+        fetched++;
+      }
+    };
     const int lim = row < nrows ? sight.limit(row / p.G) : 0;
-    const uint32_t mine = (uint32_t)(warp * 32) << 16;
+    const uint32_t mine = (uint32_t)(quad * 32) << 16;
     // what the tile before gave joins the running result, and both go to the new reference: the tensor cores cut off what an f32
     // cannot hold, so a sum that ran on over many tiles would shrink; within a tile the residues go first
     auto sum_up = [&](bool more, float f) {
+      const uint64_t f2 = pair(f, f);
 #pragma unroll 1
-      for (int c = 0; c < HDP; c += 16) {
+      for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
         uint32_t x[16], y[16];
         tc::tmem_ld16(tO + mine + c, x);
         if (more) tc::tmem_ld16(tSum + mine + c, y);
         tc::tmem_ld_wait();
-        if (more) {
 #pragma unroll
-          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(x[e]));
+        for (int e = 0; e < 16; e += 2) {
+          uint64_t v = pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          if (more) v = add2(v, pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])));
+          const float2 r = unpair(mul2(v, f2));
+          x[e] = __float_as_uint(r.x), x[e + 1] = __float_as_uint(r.y);
         }
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
         tmem_st16(tSum + mine + c, x);
       }
     };
-    for (int k = 0; k < nt && ok; k++) {
-      ok = wait(s_full, k & 1);
-      if (!__all_sync(0xffffffffu, ok)) break;
+    if (nt > 0) keys(0), values(0);
+    for (int k = 0; k < nt; k++) {
+      wait(s_full, k & 1);
+      __syncwarp();
       tc::tc_fence_after();
-      const int first = (t0 + k) * kTile;
+      const int seen = lim - (t0 + k) * kTile - 64 * half;  // of this thread's 64 positions
       float top = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < 4; c++) {
+      for (int c = 0; c < 2; c++) {
         float v[32];
-        tmem_ld32(tS + mine + 32 * c, v);
-        const int n = lim - first - 32 * c;
+        tmem_ld32(tS + mine + 64 * half + 32 * c, v);
+        const int n = seen - 32 * c;
         float t = -INFINITY;
         if (__all_sync(0xffffffffu, n >= 32)) {
 #pragma unroll
-          for (int e = 0; e < 32; e++) t = fmaxf(t, v[e]);
+          for (int e = 0; e < 32; e += 4) t = max3(t, fmaxf(v[e], v[e + 1]), fmaxf(v[e + 2], v[e + 3]));
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e++) t = e < n ? fmaxf(t, v[e]) : t;
         }
-        if (n > 0) top = fmaxf(top, t * (scl[k & 1][c][0] * kScoreUnit * qs));
+        if (n > 0) top = fmaxf(top, t * (scl[k & 1][2 * half + c][0] * qs));
       }
+      // the row's maximum: the other half's too
+      tops[k & 1][half][local] = top;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
+      top = fmaxf(top, tops[k & 1][1 - half][local]);
       // a new reference where the maximum has moved far: what was summed so far is rescaled
       const bool move = top > m + kSlack || (m == -INFINITY && top > -INFINITY);
       const float old = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
@@ -977,182 +1078,165 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       if (k > 0) sum_up(k > 1, old);
       const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
-      for (int c = 0; c < 4; c++) {
+      for (int c = 0; c < 2; c++) {
         float v[32];
-        tmem_ld32(tS + mine + 32 * c, v);
-        const int n = lim - first - 32 * c;
-        const float f = scl[k & 1][c][0] * kScoreUnit * qs, wf = scl[k & 1][c][1];
-        const bool all = __all_sync(0xffffffffu, n >= 32);
         uint32_t out[32];
-        float sum0 = 0.0f, sum1 = 0.0f;
+        const uint32_t at = tS + mine + 64 * half + 32 * c;
+        tmem_ld32(at, v);
+        const int n = seen - 32 * c;
+        const float *sc = scl[k & 1][2 * half + c];
+        const float f = sc[0] * qs;
+        // weights with the values' scale in the exponent; their sum without it
+        const float shift = sc[1] - ref, inv = sc[2];
+        const uint64_t f2 = pair(f, f), shift2 = pair(shift, shift), minus = pair(-1.0f, -1.0f);
+        uint64_t sum = 0;
+        auto put = [&](int e, uint64_t w) {
+          sum = add2(sum, w);
+          const float2 x = unpair(w);
+          const __half2 hi = __floats2half2_rn(x.x, x.y);
+          const float2 back = __half22float2(hi), r = unpair(fma2(pair(back.x, back.y), minus, w));
+          out[e >> 1] = *(const uint32_t *)&hi, out[16 + (e >> 1)] = h2(r.x, r.y);
+        };
+        if (__all_sync(0xffffffffu, n >= 32)) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x = ex2(fmaf(v[e], f, -ref)), y = ex2(fmaf(v[e + 1], f, -ref));
-          if (!all) x = e < n ? x : 0.0f, y = e + 1 < n ? y : 0.0f;
-          sum0 += x, sum1 += y;
-          x *= wf, y *= wf;
-          if (!all) x = e < n ? x : 0.0f, y = e + 1 < n ? y : 0.0f;  // (a masked place's scale may be NaN)
-          split2(x, y, out[e >> 1], out[16 + (e >> 1)]);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 z = unpair(fma2(pair(v[e], v[e + 1]), f2, shift2));
+            put(e, pair(ex2(z.x), ex2(z.y)));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            put(e, pair(e < n ? ex2(fmaf(v[e], f, shift)) : 0.0f, e + 1 < n ? ex2(fmaf(v[e + 1], f, shift)) : 0.0f));
         }
-        l += sum0 + sum1;
-        tmem_st32(tS + mine + 32 * c, out);
+        const float2 both = unpair(sum);
+        if (n > 0) l = fmaf(both.x + both.y, inv, l);  // (what is not seen may have a scale that is none)
+        tmem_st32(at, out);
       }
       tmem_st_wait();
       tc::tc_fence_before();
       tc::mbar_arrive(p_full);
-    }
-    if (nt > 0 && __all_sync(0xffffffffu, ok)) ok = wait(pv_done, (nt - 1) & 1);
-    ok = __all_sync(0xffffffffu, ok);
-    tc::tc_fence_after();
-    const bool sees = lim > 0;
-    const int i = row / p.G, C = p.H * p.G * p.HD, col0 = (h * p.G + row - i * p.G) * p.HD;
-    const long long orow = (long long)s * p.T + i;
-    const float unit_of = exp2f(24 - kUpP), inv = pp.splits == 1 ? unit_of / l : unit_of;
-    const size_t part = ((size_t)unit * pp.splits + split) * nrows + row;
-    if (pp.splits > 1 && row < nrows) *(float2 *)(p.pml + part * 2) = make_float2(m, l);
-    for (int c = 0; c < HDP; c += 16) {
-      uint32_t x[16];
-      __syncwarp();
-      if (nt > 0) {
-        uint32_t y[16];
-        tc::tmem_ld16(tO + mine + c, x);
-        if (nt > 1) tc::tmem_ld16(tSum + mine + c, y);
-        tc::tmem_ld_wait();
-        if (nt > 1) {
-#pragma unroll
-          for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(x[e]));
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; e++) x[e] = nt > 0 && sees ? __float_as_uint(__uint_as_float(x[e]) * inv * svmax) : 0u;
-      float *dst = pp.splits > 1 ? p.pacc + part * HDP + c : p.out + orow * C + col0 + c;
-      if (row < nrows && (pp.splits > 1 || (p.HD % 16 == 0 && c < p.HD))) {  // whole groups of 16 channels, 64 bytes aligned
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) *(uint4 *)(dst + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-        if (p.y16 && pp.splits == 1) {
-          __half *d16 = p.y16 + ((long long)((col0 + c) >> 6) * p.R + orow) * 64 + ((col0 + c) & 63);
-          uint32_t hi[8], lo[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) split2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]), hi[e], lo[e]);
-          *(uint4 *)d16 = make_uint4(hi[0], hi[1], hi[2], hi[3]), *(uint4 *)(d16 + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-          if (p.lo_off) {
-            *(uint4 *)(d16 + p.lo_off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *(uint4 *)(d16 + p.lo_off + 8) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-          }
-        }
-      } else if (row < nrows && c < p.HD) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          if (c + e < p.HD) {
-            const float y = __uint_as_float(x[e]);
-            dst[e] = y;
-            if (p.y16) {
-              const int col = col0 + c + e;
-              __half *d16 = p.y16 + ((long long)(col >> 6) * p.R + orow) * 64 + (col & 63);
-              const __half hi = __float2half_rn(y);
-              *d16 = hi;
-              if (p.lo_off) d16[p.lo_off] = __float2half_rn(y - __half2float(hi));
-            }
-          }
-        }
+      if (k + 1 < nt) {  // the next tile, while the products run: K is free since the scores came, V when this tile's have run
+        keys(k + 1);
+        wait(pv_done, k & 1);
+        __syncwarp();
+        values(k + 1);
       }
     }
-    tc::tc_fence_before();
-  } else if (warp < 8) {  // ---- codes to tiles, a cache block per warp
-    const int w = warp - 4;
-    auto fetch = [&](int k) {  // tile k of this range into stage k & 1
-      const int b = (t0 + k) * 4, n = min(4, p.nblk - b);
-      const uint32_t bytes = (uint32_t)n * BB, dst = smem_u32(smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES), on = code_full + 8 * (k & 1);
-      tc::mbar_expect_tx(on, bytes);
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(codes + (size_t)b * BB),
-                   "r"(bytes), "r"(on)
-                   : "memory");
-    };
-    int fetched = 0;
-    if (tid == 128)
-      for (; fetched < min(2, nt); fetched++) fetch(fetched);
-    fetched = min(2, nt);
-    int k = 0;
-    for (; k < nt && ok; k++) {
-      ok = wait(code_full + 8 * (k & 1), (k >> 1) & 1);
-      const uint8_t *blk = smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES + w * BB;
-      if (k > 0) ok = ok && wait(s_full, (k - 1) & 1);  // the products of the tile before have read K
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-      for (int c = 0; c < KS; c++) {
-        const uint4 w4 = *(const uint4 *)(blk + c * 512 + lane * 16);
-        const uint32_t word[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int wi = 4 * c + u, j = wi / KS, ks = wi % KS, r = w * 32 + 8 * (g >> 1) + 2 * j + (g & 1), ch = 16 * ks + 4 * t;
-          uint2 x;
-          widen(word[u], x.x, x.y);
-          *(uint2 *)(smem + Smem::K + (ch >> 6) * 16384 + r * 128 + ((((ch & 63) >> 3) ^ (r & 7)) << 4) + (ch & 4) * 2) = x;
-        }
-      }
-      if (lane == 0) {
-        const bool there = (t0 + k) * 4 + w < p.nblk;
-        const float2 sc = there ? *(const float2 *)(blk + 2 * kBlock * HDP) : make_float2(0.f, 0.f);
-        scl[k & 1][w][0] = sc.x, scl[k & 1][w][1] = sc.y / svmax * (float)(1 << kUpP);
-      }
-      tc::fence_proxy_async_smem();
-      tc::mbar_arrive(k_full);
-      if (k > 0) ok = wait(pv_done, (k - 1) & 1);  // and V
-      if (!__all_sync(0xffffffffu, ok)) break;
-#pragma unroll
-      for (int c = 0; c < KS; c++) {
-        const uint4 w4 = *(const uint4 *)(blk + kBlock * HDP + c * 512 + lane * 16);
-        uint4 x, y;
-        widen(w4.x, x.x, x.y);
-        widen(w4.y, x.z, x.w);
-        widen(w4.z, y.x, y.y);
-        widen(w4.w, y.z, y.w);
-        const int ch = 16 * c + g, u = 4 * (w & 1) + t;  // channels ch and ch + 8, positions 32 w + 8t ..+7
-        uint8_t *dst = smem + Smem::V + (w >> 1) * (HDP * 128) + ch * 128 + ((u ^ (ch & 7)) << 4);
-        *(uint4 *)dst = x, *(uint4 *)(dst + 1024) = y;
-      }
-      tc::fence_proxy_async_smem();
-      tc::mbar_arrive(v_full);
-      tc::mbar_arrive(code_free);
-      if (fetched < nt) {
-        if (tid == 128 && wait(code_free, k & 1)) fetch(fetched);  // (where this runs out, so does the wait for the tile)
-        fetched++;
-      }
+    if (nt > 0) wait(pv_done, (nt - 1) & 1);
+    if (!ok) {
+      gave_up = 1;
+      if (tid == 0)  // one's own copies that may still be under way
+        for (int k = max(0, nt - 2); k < nt; k++) tc::mbar_wait(code_full + 8 * (k & 1), (k >> 1) & 1, p.wait_limit);
     }
-    if (!ok) gave_up = 1;
-    for (; k < fetched; k++)  // (only behind a wait that ran out) copies of one's own still under way
-      wait(code_full + 8 * (k & 1), (k >> 1) & 1);
-  } else if (lane == 0) {  // ---- products
+    tops[0][half][local] = l;
+  }
+  if (warp == 8 && lane == 0) {  // ---- products
     const uint32_t id_s = tc::make_idesc(0, kTile, kTile), id_o = tc::make_idesc(0, kTile, HDP);
-    const uint32_t q0 = smem_u32(smem + Smem::Q), k0 = smem_u32(smem + Smem::K), v0 = smem_u32(smem + Smem::V);
-    for (int k = 0; k < nt && ok; k++) {
-      ok = wait(k_full, k & 1) && (k == 0 || wait(pv_done, (k - 1) & 1));
-      if (!ok) break;
+    const uint64_t q0 = tc::smem_desc_sw128(smem_u32(smem + Smem::Q)), k0 = tc::smem_desc_sw128(smem_u32(smem + Smem::K)),
+                   v0 = tc::smem_desc_sw128(smem_u32(smem + Smem::V));  // addresses count 16 bytes, and do not carry out of their field
+    for (int k = 0; k < nt; k++) {
+      wait(k_full, k & 1);
+      if (k > 0) wait(pv_done, (k - 1) & 1);
       tc::tc_fence_after();
 #pragma unroll
       for (int part = 0; part < 2; part++)
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-          const uint32_t off = (ks >> 2) * 16384 + (ks & 3) * 32;
-          tc::umma<0>(tS, tc::smem_desc_sw128(q0 + (1 - part) * (CH * 16384) + off), tc::smem_desc_sw128(k0 + off), id_s, part + ks > 0);
+          const uint32_t off = ((ks >> 2) * 16384 + (ks & 3) * 32) / 16;
+          tc::umma<0>(tS, q0 + ((1 - part) * (CH * 16384 / 16) + off), k0 + off, id_s, part + ks > 0);
         }
       tc::umma_commit(s_full);
       tc::mbar_arrive(s_full);
-      ok = wait(v_full, k & 1) && wait(p_full, k & 1);
-      if (!ok) break;
+      wait(v_full, k & 1);
+      wait(p_full, k & 1);
       tc::tc_fence_after();
 #pragma unroll
       for (int part = 0; part < 2; part++)
 #pragma unroll
         for (int step = 0; step < 8; step++)  // 16 positions
-          umma_ts(tO, tS + (step >> 1) * 32 + (1 - part) * 16 + (step & 1) * 8, tc::smem_desc_sw128(v0 + (step >> 2) * (HDP * 128) + (step & 3) * 32),
-                  id_o, part + step > 0);
+          umma_ts(tO, tS + (step >> 1) * 32 + (1 - part) * 16 + (step & 1) * 8, v0 + ((step >> 2) * (HDP * 128) + (step & 3) * 32) / 16, id_o,
+                  part + step > 0);
       tc::umma_commit(pv_done);
     }
     if (!ok) gave_up = 1;
   }
-  if (warp < 4 && !ok) gave_up = 1;
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  // the result, through shared memory (the queries' and keys' place) so that rows are written as rows
+  constexpr int PITCH = HDP + 4;
+  float *so = (float *)smem;
+  if (warp < 8) {
+    const uint32_t mine = (uint32_t)(quad * 32) << 16;
+    const bool sees = row < nrows && sight.limit(row / p.G) > 0;
+    const float total = tops[0][0][local] + tops[0][1][local];
+    const float unit_of = exp2f(24 - kUpP), inv = pp.splits == 1 ? unit_of / total : unit_of;
+    if (pp.splits > 1 && row < nrows && half == 0)
+      *(float2 *)(p.pml + (((size_t)unit * pp.splits + split) * nrows + row) * 2) = make_float2(m, total);
+#pragma unroll 1
+    for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
+      uint32_t v[16];
+      if (nt > 0) {
+        uint32_t y[16];
+        tc::tmem_ld16(tO + mine + c, v);
+        if (nt > 1) tc::tmem_ld16(tSum + mine + c, y);
+        tc::tmem_ld_wait();
+        if (nt > 1) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(v[e]));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) v[e] = nt > 0 && sees ? __float_as_uint(__uint_as_float(v[e]) * inv * svmax) : 0u;
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) *(uint4 *)(so + local * PITCH + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    }
+    tc::tc_fence_before();
+  }
+  __syncthreads();
+  if (warp < 8 && d0 < HDP) {
+    const int C = p.H * p.G * p.HD;
+#pragma unroll 4
+    for (int k = 0; k < PER; k++) {
+      const int r = line + k * (256 / LPR);
+      if (row_a + r >= nrows) break;
+      const float4 v = *(const float4 *)(so + r * PITCH + d0);
+      if (pp.splits > 1) {
+        *(float4 *)(p.pacc + (((size_t)unit * pp.splits + split) * nrows + row_a + r) * HDP + d0) = v;
+        continue;
+      }
+      if (d0 >= p.HD) break;
+      int i, head;
+      of_row(r, i, head);
+      const long long orow = (long long)s * p.T + i;
+      const int col = head * p.HD + d0;
+      float *dst = p.out + orow * C + col;
+      if (p.HD % 4 == 0) {
+        *(float4 *)dst = v;
+        if (p.y16) {  // (four columns lie in one group of 64)
+          __half *d16 = p.y16 + ((long long)(col >> 6) * p.R + orow) * 64 + (col & 63);
+          uint2 hi, lo;
+          split2(v.x, v.y, hi.x, lo.x);
+          split2(v.z, v.w, hi.y, lo.y);
+          *(uint2 *)d16 = hi;
+          if (p.lo_off) *(uint2 *)(d16 + p.lo_off) = lo;
+        }
+      } else {
+        const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+          if (d0 + n < p.HD) {
+            dst[n] = e[n];
+            if (p.y16) {
+              __half *d16 = p.y16 + ((long long)((col + n) >> 6) * p.R + orow) * 64 + ((col + n) & 63);
+              const __half hi = __float2half_rn(e[n]);
+              *d16 = hi;
+              if (p.lo_off) d16[p.lo_off] = __float2half_rn(e[n] - __half2float(hi));
+            }
+          }
+      }
+    }
+  }
   __syncthreads();
   if (gave_up && tid == 0) {
     atomicExch(p.status, kWaits + 1);
@@ -1198,7 +1282,8 @@ int run_prompt(fa_ctx *ctx, const fa_kv8 *c, const AttnParams &a, int most, cons
   const int nrows = a.G * a.T, tiles = ceil_div(most < 1 ? 1 : most, kTile);
   pp.rowtiles = ceil_div(nrows, kTile);
   const long long blocks = (long long)c->S * c->H * pp.rowtiles, slots = (long long)ctx->sm_count * (HDP <= 64 ? 2 : 1);
-  // the positions are split while the thread blocks do not fill the GPU once, four tiles a split at least
+  // The positions are split, four tiles a split at least, while the thread blocks do not fill the GPU.  (Shorter runs of longer
+  // lists even out streams of different lengths, but cost more in queries, results and joining than that gives.)
   long long splits = blocks >= slots ? 1 : slots / blocks;
   if (splits > tiles / 4) splits = tiles / 4;
   if (splits < 1) splits = 1;
