@@ -113,6 +113,7 @@ SIGNATURES = {
     "fa_attn_kv8": [P, P, P, I, I, P, PP],
     "fa_attn_append_kv8": [P, P, P, I, I, P, P, PP],
     "fa_decoder_step": [P, P, I, P, PP, PP, PP, PP, I, I, I, P, P, P, PP],
+    "fa_decoder_step_kv8": [P, P, I, P, PP, P, I, PP, I, I, P, P, P, PP],
     "fa_conformer_block": [P, P, P, P, P, I, I, I, I, I, P, P, PP, PP],
     "fa_attn_fused": [P, P, P, P, P, P, P, I, I, I, PP],
     "fa_attn_fused_qkv": [P, P, P, P, P, I, I, I, PP],

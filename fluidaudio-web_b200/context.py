@@ -503,6 +503,15 @@ class CudaContext:
         return self._op(self._lib.fa_decoder_step, (_lib.DecoderLayer * L)(*weights), L, x.h, handles(crossK), handles(crossV),
                         handles(selfK), handles(selfV), n, NH, HD, self._live(lnf[0]), self._live(lnf[1]), C.byref(self._linear_of(logits, None)))
 
+    def decoderStepKv8(self, weights: Sequence, x, cross: Sequence[KvCache8], nCross: int, selfCaches: Sequence[KvCache8], n: int, NH: int,
+                       lnf, logits, *, lens=None) -> Tensor:
+        """Optional member: decoderStep over 8-bit caches for T >= 1 tokens of each stream, x [S*T, D] stream-major -> logits of each
+        stream's last token (see fa_decoder_step_kv8)."""
+        L = len(weights)
+        handles = lambda cs: (C.c_void_p * L)(*[c.h for c in cs])  # noqa: E731
+        return self._op(self._lib.fa_decoder_step_kv8, (_lib.DecoderLayer * L)(*weights), L, x.h, handles(cross), self._h_of(lens), nCross,
+                        handles(selfCaches), n, NH, self._live(lnf[0]), self._live(lnf[1]), C.byref(self._linear_of(logits, None)))
+
     def conformerWeights(self, w: dict):
         """The weights of conformerBlock from an encoder layer's dict of tensors (absent ones: None).  The struct holds raw
         handles: it is good while the layer's entries are the ones it was made from (engines/layer_weights.py)."""

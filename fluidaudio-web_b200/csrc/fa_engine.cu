@@ -5,7 +5,7 @@
 // entry points issue the same members in the same order (src/engines/asr-whisper/raw-whisper-decoder.js:108-140,
 // src/engines/asr-parakeet/raw-encoder.js:240-386), so that the host calls once per layer stack or block.  Nothing here
 // launches a kernel of its own and no handle is kept, views included.
-#include "fa_internal.cuh"
+#include "fa_kv8.cuh"
 
 namespace {
 
@@ -89,7 +89,45 @@ int decoder_layer(fa_ctx *ctx, const fa_decoder_layer &w, const fa_tensor *x, co
   return linear(ctx, h, nullptr, nullptr, w.f2, FA_ACT_NONE, x2, out);
 }
 
+// The same layer over 8-bit caches, for the S*T rows of T tokens per stream.
+int decoder_layer_kv8(fa_ctx *ctx, const fa_decoder_layer &w, const fa_tensor *x, fa_kv8 *cross, const fa_tensor *lens, int n_cross, fa_kv8 *self,
+                      int n, int NH, fa_tensor **out) {
+  fa_tensor *qkv, *att, *x1, *cq, *x2, *h;
+  FA_TRY(linear(ctx, x, w.ln1_w, w.ln1_b, w.sqkv, FA_ACT_NONE, nullptr, &qkv));
+  FA_TRY(fa_attn_append_kv8(ctx, qkv, self, NH, n, nullptr, nullptr, &att));
+  FA_TRY(linear(ctx, att, nullptr, nullptr, w.so, FA_ACT_NONE, x, &x1));
+  FA_TRY(linear(ctx, x1, w.ln2_w, w.ln2_b, w.cq, FA_ACT_NONE, nullptr, &cq));
+  FA_TRY(fa_attn_kv8(ctx, cq, cross, NH, n_cross, lens, &att));
+  FA_TRY(linear(ctx, att, nullptr, nullptr, w.co, FA_ACT_NONE, x1, &x2));
+  FA_TRY(linear(ctx, x2, w.ln3_w, w.ln3_b, w.f1, FA_ACT_GELU_ERF, nullptr, &h));
+  return linear(ctx, h, nullptr, nullptr, w.f2, FA_ACT_NONE, x2, out);
+}
+
 }  // namespace
+
+extern "C" int fa_decoder_step_kv8(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, const fa_tensor *x, fa_kv8 *const *cross,
+                                   const fa_tensor *lens, int n_cross, fa_kv8 *const *self, int n, int NH, const fa_tensor *lnf_w,
+                                   const fa_tensor *lnf_b, const fa_linear *logits, fa_tensor **out) {
+  if (!ctx || !out || !layers || !cross || !self || !logits) return fa_fail(ctx, FA_ERR_INVALID, "decoderStepKv8: NULL argument");
+  *out = nullptr;
+  FA_REQUIRE(ctx, fa_valid(ctx, x) && n_layers > 0 && fa_valid_kv8(ctx, self[0]), "decoderStepKv8: unknown handle");
+  const int S = self[0]->S, T = x->rows / S, D = x->cols;
+  FA_REQUIRE(ctx, T >= 1 && x->rows % S == 0, "decoderStepKv8: %d rows for %d streams", x->rows, S);
+  ArenaScope scope(ctx);
+  FA_TRY(scope.open());
+  fa_tensor *cur = nullptr, *y = nullptr;
+  for (int l = 0; l < n_layers; l++) FA_TRY(decoder_layer_kv8(ctx, layers[l], cur ? cur : x, cross[l], lens, n_cross, self[l], n, NH, &cur));
+  Views views(ctx);
+  if (T > 1) {  // the last token of each stream
+    fa_tensor *wide;
+    FA_TRY(views.reshape(cur, S, T * D, &wide));
+    FA_TRY(fa_slice_cols(ctx, wide, (T - 1) * D, D, &cur));
+  }
+  FA_TRY(linear(ctx, cur, lnf_w, lnf_b, *logits, FA_ACT_NONE, nullptr, &y));
+  FA_TRY(fa_pin(ctx, y, 1));
+  *out = y;
+  return FA_OK;
+}
 
 extern "C" int fa_decoder_step(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, const fa_tensor *x, fa_tensor *const *cross_k,
                                fa_tensor *const *cross_v, fa_tensor *const *self_k, fa_tensor *const *self_v, int n, int NH, int HD,

@@ -19,6 +19,11 @@ Two drivers share the weights:
     attention is the SAME member with H = S*NH "heads"; of the plain sequence only reshapeView is outside
     the reference interface (a JS engine re-labels {rows, cols} for that).
 Both produce the same logits row for a stream; the tests hold them to the CPU reference's token ids.
+
+With cache="int8" (backends with the 8-bit cache members) the S-stream driver keeps all keys and values as 8-bit codes with a
+scale for each block of 32 positions and head: a quarter of the f32 caches' memory and of what a step reads.  Streams may then
+have encoder outputs of different lengths, and prompts go through the layers in one step (prefill_streams).  `rules` are the
+keyword arguments of pickAdjusted (penalties for tokens picked so far, a bias, a mask of allowed tokens).
 """
 from __future__ import annotations
 
@@ -193,12 +198,45 @@ def _layer(ctx, x, w, kv, cacheK, cacheV, n, S, D, NH, HD):
     return _linear(ctx, h, w["f2w"], bias=w["f2b"], add=x)
 
 
+def _layer_kv8(ctx, x, w, kv, cache, n, NH):
+    """The same layer over 8-bit caches, x [S*T, D] being T tokens of each stream from position n on."""
+    if fused_from(w, "sqkvw", QKV_PARTS):
+        qkv = _linear(ctx, x, w["sqkvw"], norm=w["ln1"], bias=w["sqkvb"])
+    else:
+        h = ctx.layernorm(x, *w["ln1"])
+        qkv = ctx.alloc(x.rows, 3 * x.cols)
+        for i, part in enumerate((_mm(ctx, h, w["sqw"], bias=w["sqb"]), _mm(ctx, h, w["skw"]), _mm(ctx, h, w["svw"], bias=w["svb"]))):
+            ctx.setCols(qkv, part, i * x.cols)
+    x = _linear(ctx, ctx.attnAppendKv8(qkv, cache, NH, n), w["sow"], bias=w["sob"], add=x)
+    cq = _linear(ctx, x, w["cqw"], norm=w["ln2"], bias=w["cqb"])
+    x = _linear(ctx, ctx.attnKv8(cq, kv["cache"], NH, kv["n"], lens=kv["lens"]), w["cow"], bias=w["cob"], add=x)
+    h = _linear(ctx, x, w["f1w"], norm=w["ln3"], bias=w["f1b"], act="gelu_erf")
+    return _linear(ctx, h, w["f2w"], bias=w["f2b"], add=x)
+
+
+def _step_kv8(ctx, dec, kv, st, x, n, S, native):
+    cfg = dec["cfg"]
+    if None not in native and hasattr(ctx, "decoderStepKv8"):
+        return ctx.decoderStepKv8(native, x, [c["cache"] for c in kv], kv[0]["n"], st["self8"], n, cfg["NH"], dec["lnf"], dec["embedT"].native(),
+                                  lens=kv[0]["lens"])
+    T = x.rows // S
+    for li, w in enumerate(dec["layers"]):
+        x = _layer_kv8(ctx, x, w, kv[li], st["self8"][li], n, cfg["NH"])
+    if T > 1:  # the last token of each stream
+        x = ctx.sliceCols(ctx.reshapeView(x, S, T * cfg["D"]), (T - 1) * cfg["D"], cfg["D"])
+    return _linear(ctx, x, dec["embedT"], norm=dec["lnf"])
+
+
 def _step(ctx, dec, kv, st, x, n, S):
     """The device part of one token: x [S, D] (embedding + position n) -> logits [S, VOCABP]."""
     cfg = dec["cfg"]
     D, NH, HD = cfg["D"], cfg["NH"], cfg["HD"]
     make = _native_of(ctx)
     native = [native_struct(w, NATIVE_KEYS, make) if "native" in w else None for w in dec["layers"]]
+    if ("self8" in st) != ("cache" in kv[0]):
+        raise ValueError("8-bit self-attention caches go with 8-bit cross-attention caches")
+    if "self8" in st:
+        return _step_kv8(ctx, dec, kv, st, x, n, S, native)
     if None not in native:
         return ctx.decoderStep(native, x, [c["k"] for c in kv], [c["v"] for c in kv], st["selfK"],
                                st["selfV"], n, NH, HD, dec["lnf"], dec["embedT"].native())
@@ -271,21 +309,50 @@ def greedy_decode(ctx, dec, enc, prefix: Sequence[int], n_tokens: int, margins: 
 
 # ---------------------------------------------------------------------------- S streams in lock step
 
-def cross_kv_streams(ctx, dec, encs) -> list:
+def cross_kv_streams(ctx, dec, encs, cache: Optional[str] = None, S: int = 0, lens=None) -> list:
     """Cross K/V of S clips in ONE product per matrix: the clips' encoder outputs stacked along rows,
     [S*Tenc, D] (a list of [Tenc, D] tensors is concatenated), give k, v [S*Tenc, D] - which is the
-    windowed operand layout of bmmQK / bmmPV with W = S."""
-    enc_all = ctx.concatRows(list(encs)) if isinstance(encs, (list, tuple)) else encs
+    windowed operand layout of bmmQK / bmmPV with W = S.
+
+    cache="int8" codes them into 8-bit caches (give them back with free_caches).  `encs` is then a list, or one tensor with
+    S; `lens` [S] (a device tensor) says how many rows of each clip are there, the rest being padding that nobody sees."""
+    stacked = isinstance(encs, (list, tuple))
+    S = len(encs) if stacked else S
+    enc_all = ctx.concatRows(list(encs)) if stacked else encs
     out = []
+    if cache not in (None, "int8"):
+        raise ValueError(f"cross_kv_streams: cache {cache!r}")
+    if cache and (S < 1 or enc_all.rows % S):
+        raise ValueError(f"cross_kv_streams: {enc_all.rows} rows for {S} clips")
+    if lens is not None and not cache:
+        raise ValueError("cross_kv_streams: lengths of the clips' own need 8-bit caches")
+    cfg = dec["cfg"]
     for w in dec["layers"]:
         k = ctx.pin(_mm(ctx, enc_all, w["ckw"]))
         v = ctx.pin(_mm(ctx, enc_all, w["cvw"], bias=w["cvb"]))
-        out.append(dict(k=k, v=v))
+        if cache:
+            n = enc_all.rows // S
+            c = ctx.kvWrite8(ctx.kvCache8(S, n, cfg["NH"], cfg["HD"]), k, v, counts=lens)
+            ctx.freeTensor(k)
+            ctx.freeTensor(v)
+            out.append(dict(cache=c, n=n, lens=lens))
+        else:
+            out.append(dict(k=k, v=v))
     return out
 
 
-def decode_init_streams(ctx, dec, S: int, maxLen: int = 448) -> dict:
+def free_caches(ctx, kv: Optional[list] = None, st: Optional[dict] = None) -> None:
+    """Gives the 8-bit caches of cross_kv_streams and decode_init_streams back."""
+    for c in [e["cache"] for e in kv or [] if "cache" in e] + (st or {}).get("self8", []):
+        ctx.freeKvCache8(c)
+
+
+def decode_init_streams(ctx, dec, S: int, maxLen: int = 448, cache: Optional[str] = None) -> dict:
     D = dec["cfg"]["D"]
+    if cache == "int8":
+        return dict(n=0, S=S, maxLen=maxLen, self8=[ctx.kvCache8(S, maxLen, dec["cfg"]["NH"], dec["cfg"]["HD"]) for _ in dec["layers"]])
+    if cache is not None:
+        raise ValueError(f"decode_init_streams: cache {cache!r}")
     return dict(n=0, S=S, maxLen=maxLen, selfK=[ctx.pin(ctx.alloc(maxLen, S * D)) for _ in dec["layers"]],
                 selfV=[ctx.pin(ctx.alloc(maxLen, S * D)) for _ in dec["layers"]])
 
@@ -296,23 +363,54 @@ def step_streams(ctx, dec, kv, st, x, n: int):
     return _step(ctx, dec, kv, st, x, n, st["S"])
 
 
-def decode_next_streams(ctx, dec, kv, st, tokens: Sequence[int], want_logits: bool = False):
+def _pick(ctx, st, logits, VOCAB, rules):
+    """The next token of each stream on the device: [S, 2] = {index, value}.  Under `rules` the picks so far (st["hist"],
+    [rows, S], its first st["picked"] rows) are the history, and the pick joins it."""
+    if rules is None:
+        return ctx.argmaxRowsIndex(logits, VOCAB)
+    if "hist" not in st:
+        st["hist"], st["picked"] = ctx.pin(ctx.alloc(st["maxLen"], st["S"])), 0
+    pick = ctx.pickAdjusted(logits, VOCAB, history=st["hist"], n=st["picked"], **rules)
+    ctx.copyRows(st["hist"], ctx.reshapeView(ctx.sliceCols(pick, 0, 1), 1, st["S"]), st["picked"])
+    st["picked"] += 1
+    return pick
+
+
+def decode_next_streams(ctx, dec, kv, st, tokens: Sequence[int], want_logits: bool = False, rules: Optional[dict] = None):
     """One token per stream.  Returns (next token ids [S] by first-maximum argmax over the VOCAB real
     columns, logits [S, VOCAB] or None).  The token pick runs on the device when the backend has
-    argmaxRowsIndex (8 bytes per stream come back instead of a logits row), else on the host."""
+    argmaxRowsIndex (8 bytes per stream come back instead of a logits row), else on the host.  With `rules` the pick is
+    pickAdjusted's (its history: the tokens that calls with rules have picked on this state so far); a stream that may pick
+    nothing gets -1."""
+    return prefill_streams(ctx, dec, kv, st, np.asarray(tokens, dtype=np.int64).reshape(-1, 1), want_logits, rules)
+
+
+def prefill_streams(ctx, dec, kv, st, tokens, want_logits: bool = False, rules: Optional[dict] = None):
+    """T tokens of each stream, tokens [S, T], in one step (T > 1 needs 8-bit caches): returns what decode_next_streams
+    returns for the last of them."""
     cfg = dec["cfg"]
     D, VOCAB = cfg["D"], cfg["VOCAB"]
     S, n = st["S"], st["n"]
-    emb = dec["embed"][np.asarray(tokens, dtype=np.int64)] + dec["pos"][n][None, :]
-    x = ctx.upload(np.ascontiguousarray(emb, dtype=f32), S, D)
+    tokens = np.asarray(tokens, dtype=np.int64)
+    T = tokens.shape[1]
+    if tokens.shape[0] != S or T < 1:
+        raise ValueError(f"prefill_streams: tokens of shape {tokens.shape} for {S} streams")
+    if T > 1 and "self8" not in st:
+        raise ValueError("prefill_streams: several tokens in one step need 8-bit caches")
+    if tokens.min() < 0:
+        raise ValueError("prefill_streams: a token id below 0 (a stream whose rules allowed no token)")
+    if rules is not None and want_logits:
+        raise ValueError("prefill_streams: rules are for the pick on the device")
+    emb = dec["embed"][tokens] + dec["pos"][n:n + T][None, :, :]
+    x = ctx.upload(np.ascontiguousarray(emb, dtype=f32), S * T, D)
     arena = ctx.pushArena()
     on_device = hasattr(ctx, "argmaxRowsIndex") and not want_logits
 
     def body():
         logits = step_streams(ctx, dec, kv, st, x, n)
-        st["n"] = n + 1
+        st["n"] = n + T
         if on_device:
-            return ctx.stageDownload(ctx.argmaxRowsIndex(logits, VOCAB))
+            return ctx.stageDownload(_pick(ctx, st, logits, VOCAB, rules))
         return ctx.stageDownload(logits)
 
     try:
@@ -328,22 +426,32 @@ def decode_next_streams(ctx, dec, kv, st, tokens: Sequence[int], want_logits: bo
 
 
 def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tokens: int,
-                          kv=None, st=None) -> np.ndarray:
+                          kv=None, st=None, cache: Optional[str] = None, lens=None, rules: Optional[dict] = None) -> np.ndarray:
     """S clips decoded in lock step: the forced prefix, then n_tokens greedy tokens per stream.
-    Returns int64 [S, n_tokens]."""
+    Returns int64 [S, n_tokens].  cache="int8": caches made here are 8-bit ones, and a state with such caches takes the prefix
+    in one step; `lens` as in cross_kv_streams, `rules` as in decode_next_streams (the history: the tokens picked here)."""
     S = len(encs)
-    kv = kv if kv is not None else cross_kv_streams(ctx, dec, encs)
-    st = st if st is not None else decode_init_streams(ctx, dec, S, len(prefix) + n_tokens)
-    st["n"] = 0
-    nxt = None
-    for t in prefix:
-        nxt, _ = decode_next_streams(ctx, dec, kv, st, [int(t)] * S)
-    out = np.empty((S, n_tokens), np.int64)
-    for i in range(n_tokens):
-        out[:, i] = nxt
-        if i + 1 < n_tokens:
-            nxt, _ = decode_next_streams(ctx, dec, kv, st, nxt)
-    return out
+    own_kv, own_st = kv is None, st is None
+    kv = cross_kv_streams(ctx, dec, encs, cache, lens=lens) if own_kv else kv
+    st = decode_init_streams(ctx, dec, S, len(prefix) + n_tokens, cache) if own_st else st
+    st["n"] = st["picked"] = 0
+    try:
+        nxt = None
+        if "self8" in st:
+            nxt, _ = prefill_streams(ctx, dec, kv, st, np.tile(np.asarray(prefix, np.int64), (S, 1)), rules=rules)
+        else:
+            for i, t in enumerate(prefix):
+                nxt, _ = decode_next_streams(ctx, dec, kv, st, [int(t)] * S, rules=rules if i + 1 == len(prefix) else None)
+        out = np.empty((S, n_tokens), np.int64)
+        for i in range(n_tokens):
+            out[:, i] = nxt
+            if i + 1 < n_tokens:
+                nxt, _ = decode_next_streams(ctx, dec, kv, st, nxt, rules=rules)
+        return out
+    finally:
+        free_caches(ctx, kv if own_kv else None, st if own_st else None)
+        if own_st and "hist" in st:
+            ctx.freeTensor(st["hist"])
 
 
 # ---------------------------------------------------------------------------- device-resident greedy loop
@@ -358,13 +466,13 @@ def resident_tables(ctx, dec) -> dict:
     return dec
 
 
-def greedy_decode_streams_resident(ctx, dec, enc_all, S: int, prefix_idx: Sequence, n_tokens: int, st=None):
+def greedy_decode_streams_resident(ctx, dec, enc_all, S: int, prefix_idx: Sequence, n_tokens: int, st=None, rules: Optional[dict] = None):
     """The whole lock-step greedy decode enqueued with no host round trip: token pick (argmaxRowsIndex)
     and the next token's embedding gather (embedRows) stay on the device, so the sequence of all
     len(prefix)+n_tokens-1 steps can also be recorded once and replayed.  `prefix_idx` holds one device
     tensor [S,1] of token ids per forced prefix position.  Returns the device tensor [n_tokens, S] of
     token ids (as floats).  Needs the backend's optional members; same arithmetic as
-    decode_next_streams."""
+    decode_next_streams.  `rules` as there; a stream that may pick nothing is reported by the next sync."""
     cfg = dec["cfg"]
     VOCAB = cfg["VOCAB"]
     resident_tables(ctx, dec)
@@ -375,10 +483,14 @@ def greedy_decode_streams_resident(ctx, dec, enc_all, S: int, prefix_idx: Sequen
     try:
         pick = None
         n = 0
+
+        def choose(logits, picked):
+            return ctx.argmaxRowsIndex(logits, VOCAB) if rules is None else ctx.pickAdjusted(logits, VOCAB, history=hist, n=picked, **rules)
+
         for idx in prefix_idx:
             step = ctx.pushArena()
             x = ctx.embedRows(dec["embedDev"], dec["posDev"], idx, n)
-            pick = ctx.argmaxRowsIndex(step_streams(ctx, dec, kv, st, x, n), VOCAB)
+            pick = choose(step_streams(ctx, dec, kv, st, x, n), 0)
             ctx.pin(pick, True)
             ctx.popArena(step)
             n += 1
@@ -388,7 +500,7 @@ def greedy_decode_streams_resident(ctx, dec, enc_all, S: int, prefix_idx: Sequen
                 break
             step = ctx.pushArena()
             x = ctx.embedRows(dec["embedDev"], dec["posDev"], pick, n)
-            pick = ctx.argmaxRowsIndex(step_streams(ctx, dec, kv, st, x, n), VOCAB)
+            pick = choose(step_streams(ctx, dec, kv, st, x, n), i + 1)
             ctx.pin(pick, True)
             ctx.popArena(step)
             n += 1

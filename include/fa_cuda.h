@@ -314,6 +314,12 @@ typedef struct fa_decoder_layer { /* raw-whisper-decoder.js:38-61; sqkv = self-a
 int fa_decoder_step(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, const fa_tensor *x, fa_tensor *const *cross_k,
                     fa_tensor *const *cross_v, fa_tensor *const *self_k, fa_tensor *const *self_v, int n, int NH, int HD,
                     const fa_tensor *lnf_w, const fa_tensor *lnf_b, const fa_linear *logits, fa_tensor **out);
+/* The same over 8-bit caches, for T >= 1 tokens of each of S streams (a prompt, or one token): x [S*T, D], stream-major, tokens
+ * at positions n .. n+T-1 -> logits of each stream's last token [S, N].  cross, self: one cache per layer; the cross caches
+ * hold n_cross positions, or lens[s] of them (fa_attn_kv8). */
+int fa_decoder_step_kv8(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, const fa_tensor *x, fa_kv8 *const *cross,
+                        const fa_tensor *lens, int n_cross, fa_kv8 *const *self, int n, int NH, const fa_tensor *lnf_w,
+                        const fa_tensor *lnf_b, const fa_linear *logits, fa_tensor **out);
 typedef struct fa_feed_forward {
   const fa_tensor *ln_w, *ln_b;
   fa_tensor *w1, *w2;
