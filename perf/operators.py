@@ -271,13 +271,14 @@ def _context():
 
 
 class _Buffer:
-    def __init__(self, ptr, shape, f16):
+    def __init__(self, ptr, shape, f16, owner=None):
+        self.owner = owner  # the memory goes back to the context with it: a result keeps it
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "typestr": "<f2" if f16 else "<f4", "version": 3}
 
 
-def _view(ctx, t):
+def _view(ctx, t, owner=None):
     """A tensor of the context as a torch tensor on the same memory."""
-    return torch.as_tensor(_Buffer(ctx.devicePtr(t), (t.rows, t.cols), t.f16), device="cuda")
+    return torch.as_tensor(_Buffer(ctx.devicePtr(t), (t.rows, t.cols), t.f16, owner), device="cuda")
 
 
 def _tensor(ctx, values):
@@ -312,7 +313,7 @@ class _Held:
 
     def give(self, t):
         self.out.append(t)
-        return _view(self.ctx, t)
+        return _view(self.ctx, t, self)
 
     def __del__(self):
         try:
