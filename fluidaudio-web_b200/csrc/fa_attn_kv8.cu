@@ -75,9 +75,12 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
   hi = *(const uint32_t *)&h;
   lo = h2(a - f.x, b - f.y);
 }
-// A word of four codes as two pairs of f16 subnormals, code * 2^-24 (see fa_kv8.cuh).
+// A word of four codes as two pairs of f16 u - 128.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t &b0, uint32_t &b1) {
-  b0 = w & 0x807F807Fu, b1 = __byte_perm(w, 0u, 0x2301) & 0x807F807Fu;
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+  const uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 p = __hsub2(*(const __half2 *)&x, bias), q = __hsub2(*(const __half2 *)&y, bias);
+  b0 = *(const uint32_t *)&p, b1 = *(const uint32_t *)&q;
 }
 // two f32 at once
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -113,10 +116,10 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^(m - M) for M >= m, 1 where the two are the same infinity
 __device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.0f : ex2(m - M); }
 
-// Weights and query rows are scaled by 2^kUp before they are split (f16 ends at 2^16), codes are 2^-24 times themselves.
+// Weights and query rows are scaled by 2^kUp before they are split (f16 ends at 2^16, and the less of a residue is subnormal the
+// better); the weights' is in their sum too.
 constexpr int kUp = 14;
-constexpr float kScoreUnit = 1024.0f * kLog2e;  // 2^(24 - kUp), scores in units of log 2
-constexpr float kValueUnit = 16777216.0f;       // 2^24; the weights' 2^kUp is in their sum too
+constexpr float kScoreUnit = kLog2e / (1 << kUp);  // scores in units of log 2
 
 // Channels 16k + 4t ..+3 of query row `row` for all k, scaled by the power of two that brings its largest element to
 // [2^kUp, 2^(kUp+1)); returns 2^kUp over that scale, NaN for a row that is not finite.  The four lanes of a quad hold the row.
@@ -433,7 +436,7 @@ struct Joined {
   __device__ __forceinline__ void finish(const AttnParams &p, int s, int h, int row, bool sees, int lane) const {
     const int i = row / p.G, C = p.H * p.G * p.HD, col0 = (h * p.G + row - i * p.G) * p.HD;
     const long long orow = (long long)s * p.T + i;
-    const float inv = kValueUnit / L;
+    const float inv = 1.0f / L;
 #pragma unroll
     for (int k = 0; k < HDP / 32; k++) {
       const int d = lane + 32 * k, col = col0 + d;
@@ -1170,7 +1173,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
     const uint32_t mine = (uint32_t)(quad * 32) << 16;
     const bool sees = row < nrows && sight.limit(row / p.G) > 0;
     const float total = tops[0][0][local] + tops[0][1][local];
-    const float unit_of = exp2f(24 - kUpP), inv = pp.splits == 1 ? unit_of / total : unit_of;
+    const float unit_of = 1.0f / (1 << kUpP), inv = pp.splits == 1 ? unit_of / total : unit_of;
     if (pp.splits > 1 && row < nrows && half == 0)
       *(float2 *)(p.pml + (((size_t)unit * pp.splits + split) * nrows + row) * 2) = make_float2(m, total);
 #pragma unroll 1
@@ -1268,7 +1271,6 @@ __global__ void __launch_bounds__(kThreads) k_join_kv8(const AttnParams p, int s
     for (int i = 0; i < HDP / 32; i++) v[i] = p.pacc[part * HDP + lane + 32 * i];
     j.add(ml.x, ml.y, v);
   }
-  j.L *= kValueUnit;  // (these parts are in the values' own unit)
   j.finish(p, s, h, row, sight.limit(row / p.G) > 0, lane);
 }
 

@@ -51,7 +51,7 @@ __device__ __forceinline__ float load1(const float *p) { return *p; }
 __device__ __forceinline__ float load1(const __half *p) { return __half2float(*p); }
 
 __device__ __noinline__ uint32_t exact_code(float x, float scale) {
-  return scale > 0.0f && scale < INFINITY ? (uint32_t)min(rint(fabs((double)x) / (double)scale), 127.0) : 0u;
+  return scale > 0.0f && scale < INFINITY ? (uint32_t)(128 + (int)fmin(fmax(rint((double)x / (double)scale), -127.0), 127.0)) : 128u;
 }
 
 // The word of four values.  The quotient's integer is taken from the product with 1 / scale, off by less than 2.4e-5 at most
@@ -59,13 +59,14 @@ __device__ __noinline__ uint32_t exact_code(float x, float scale) {
 // take the f64 quotient, which never rounds across a tie (x and scale have 24 bits each).
 __device__ __forceinline__ uint32_t code4(float x0, float x1, float x2, float x3, float scale, float inv) {
   const float x[4] = {x0, x1, x2, x3};
+  constexpr float kMagic = 12583040.0f;  // 1.5 * 2^23 + 128: the sum's low byte is the nearest integer + 128, ties to even
   uint32_t u[4];
   float off = 0.0f;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const float a = fabsf(x[e]) * inv, r = a + 8388608.0f;  // 2^23: the sum's low bits are the nearest integer, ties to even
+    const float t = x[e] * inv, r = t + kMagic;
     u[e] = __float_as_uint(r);
-    off = fmaxf(off, fabsf(a - (r - 8388608.0f)));
+    off = fmaxf(off, fabsf(t - (r - kMagic)));
   }
   if (!(off < 0.49997f) || !(scale > 1e-30f && scale < INFINITY)) {
 #pragma unroll 1
@@ -77,10 +78,7 @@ __device__ __forceinline__ uint32_t code4(float x0, float x1, float x2, float x3
       if (e == 3) u[3] = q;
     }
   }
-  const uint32_t mag = __byte_perm(__byte_perm(u[0], u[2], 0x0040), __byte_perm(u[1], u[3], 0x0040), 0x5410);
-  const uint32_t sign = __byte_perm(__byte_perm(__float_as_uint(x[2]), __float_as_uint(x[0]), 0x0073),
-                                    __byte_perm(__float_as_uint(x[3]), __float_as_uint(x[1]), 0x0073), 0x5410);
-  return mag | (sign & 0x80808080u);
+  return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
 }
 
 // One block, keys (WHICH = 0) or values (1): rows to registers, their largest magnitude, codes to shared memory in the block's
@@ -246,11 +244,10 @@ struct ReadParams {
   int row0, rows, H, HD, nblk;
 };
 
-// A word of codes as four values: the codes come as f16 subnormals, whole numbers after the exact product with 2^24.
+// A word of codes as four values.
 __device__ __forceinline__ float4 values4(uint32_t w, float scale) {
-  const uint32_t a = w & 0x807F807Fu, b = __byte_perm(w, 0u, 0x2301) & 0x807F807Fu;
-  const float2 x = __half22float2(*(const __half2 *)&a), y = __half22float2(*(const __half2 *)&b);
-  return make_float4(x.x * 16777216.0f * scale, x.y * 16777216.0f * scale, y.x * 16777216.0f * scale, y.y * 16777216.0f * scale);
+  auto one = [&](uint32_t selector) { return (__uint_as_float(__byte_perm(w, 0x4B000000u, selector)) - 8388736.0f) * scale; };  // 2^23 + u
+  return make_float4(one(0x7540), one(0x7541), one(0x7542), one(0x7543));
 }
 
 // One half of a block: a thread turns one word of keys, or four words of values, into four values of a row, or of four rows.

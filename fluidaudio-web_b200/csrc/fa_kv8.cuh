@@ -1,13 +1,11 @@
 // The 8-bit key and value cache: layout and device helpers shared by the kernels that write and read it.
 //
 // A block holds 32 consecutive positions of one head of one stream: K 32 x HDP codes, V 32 x HDP codes, then the two scales.
-// A code is q = rint(x / scale) in -127..127 with scale = max|x| / 127 over the rows that the block holds, so x is read as
-// q * scale: one rounding, half a step of the block's largest value / 127 at most.
-//
-// Codes are signs and magnitudes, four to a word in an order that makes them f16 operands with three instructions: an f16 with
-// a zero exponent is a whole number times 2^-24, so sign (bit 15) and magnitude (bits 0..6) ARE the code.  Each half of a word
-// holds one code that way, and a second one with its sign in bit 7 and its magnitude in bits 8..14, which is the first kind
-// once the half's bytes change places: codes 0 and 1 of the word are the halves' first, 2 and 3 their second ones.
+// A code is u = q + 128 with q = rint(x / scale) in -127..127 and scale = max|x| / 127 over the rows that the block holds, so
+// x is read as (u - 128) * scale: one rounding, half a step of the block's largest value / 127 at most.  0x6400 | u is the f16
+// 1024 + u, so two codes become f16 operands u - 128 with a byte permutation and a subtraction.  (Signs and magnitudes would be
+// f16 subnormals as they stand, an instruction less a word; but the tensor cores align products by exponent fields, and the
+// leading zeros of subnormals cost the sums three bits and more: 3e-6 instead of 3e-7 from float64.)
 //
 // The codes lie in the order in which the lanes of a warp take them as operands of m16n8k16 products (B fragments: lane
 // (g, t) = (lane / 4, lane % 4) holds column g and k = 2t, 2t+1, 2t+8, 2t+9), 16 bytes a lane and 512 a warp:
@@ -29,10 +27,7 @@ inline int stored_width(int HD) { return HD <= 32 ? 32 : HD <= 64 ? 64 : HD <= 9
 __host__ __device__ constexpr size_t block_bytes(int HDP) { return (size_t)2 * kBlock * HDP + 16; }
 
 // code e of a word
-__device__ __forceinline__ float unpack(uint32_t w, int e) {
-  const uint32_t half = w >> (16 * (e & 1)), mag = half >> (e < 2 ? 0 : 8) & 0x7f, sign = half >> (e < 2 ? 15 : 7) & 1;
-  return sign ? -(float)mag : (float)mag;
-}
+__device__ __forceinline__ float unpack(uint32_t w, int e) { return (float)((int)(w >> (8 * e) & 255u) - 128); }
 
 // Where stream s's new rows go: `start` = pos[s] or n, `count` = counts[s] or T rows, both inside the cache.
 struct Rows {
