@@ -127,6 +127,14 @@ class CudaContext:
         self._check(fn(self._h, *args, C.byref(out)))
         return self._wrap(out)
 
+    def _op_f32(self, rows: int, cols: int, fn, *args) -> Tensor:
+        """_op of a member whose result is [rows, cols] in f32 (asking the library for that costs 1.5 us of host time)."""
+        out = C.c_void_p()
+        rc = fn(self._h, *args, C.byref(out))
+        if rc != 0:
+            self._check(rc)
+        return Tensor(out.value, rows, cols)
+
     # -- tensors & memory (compute.d.ts:109-133) ------------------------------------------------
     def upload(self, data, rows: int, cols: int) -> Tensor:
         a = _np_f32(data)
@@ -457,17 +465,18 @@ class CudaContext:
         """Positions row0..row0+rows-1 as the values that are stored: (k, v) [S*rows, H*HD]."""
         k, v = C.c_void_p(), C.c_void_p()
         self._check(self._lib.fa_kv8_read(self._h, cache.h, row0, rows, C.byref(k), C.byref(v)))
-        return self._wrap(k), self._wrap(v)
+        n, w = cache.S * rows, cache.H * cache.HD
+        return Tensor(k.value, n, w), Tensor(v.value, n, w)
 
     def attnKv8(self, q, cache: KvCache8, HQ: int, n: int, *, lens=None) -> Tensor:
         """softmax(q K^T) V over the cache's first n positions (or lens [S] of them) for T queries per stream, q [S*T, HQ*HD];
         HQ / H neighbouring query heads share a key head.  A stream of length 0 gives zeros."""
-        return self._op(self._lib.fa_attn_kv8, q.h, cache.h, HQ, n, self._h_of(lens))
+        return self._op_f32(q.rows, q.cols, self._lib.fa_attn_kv8, q.h, cache.h, HQ, n, self._h_of(lens))
 
     def attnAppendKv8(self, qkv, cache: KvCache8, HQ: int, n: int = 0, *, pos=None, counts=None) -> Tensor:
         """The self-attention form: qkv [S*T, (HQ+2H)*HD] = q | k | v of T new tokens per stream; k and v go to positions
         n..n+T-1 (pos, counts as in kvWrite8), query i attends over positions 0..n+i.  Rows from counts[s] on give zeros."""
-        return self._op(self._lib.fa_attn_append_kv8, qkv.h, cache.h, HQ, n, self._h_of(pos), self._h_of(counts))
+        return self._op_f32(qkv.rows, HQ * cache.HD, self._lib.fa_attn_append_kv8, qkv.h, cache.h, HQ, n, self._h_of(pos), self._h_of(counts))
 
     # -- layer loops in native code (optional members) -----------------------------------------------
     @staticmethod
@@ -615,13 +624,13 @@ class CudaContext:
         """Optional member: penalties for the tokens of the first n rows of `history` [>=n, rows], a bias [1 or rows, ncols] and a
         mask of allowed tokens (rows of ceil(ncols/32) little-endian 32-bit words; maskRows [rows] says which row each goes by)
         -> [rows, ncols] logits, -inf where a token is not allowed (see fa_logit_rules)."""
-        return self._op(self._lib.fa_adjust_logits, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
+        return self._op_f32(x.rows, ncols if ncols > 0 else x.cols, self._lib.fa_adjust_logits, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
 
     def pickAdjusted(self, x, ncols: int = 0, *, history=None, n: int = 0, repetition: float = 1.0, presence: float = 0.0,
                      frequency: float = 0.0, bias=None, mask: Optional[PackedBytes] = None, maskRows=None) -> Tensor:
         """Optional member: argmaxRowsIndex of adjustLogits in one pass: [rows, 2] = {index, value}, {-1, -inf} for a row in which
         no token is allowed."""
-        return self._op(self._lib.fa_pick_adjusted, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
+        return self._op_f32(x.rows, 2, self._lib.fa_pick_adjusted, x.h, ncols, self._rules(history, n, repetition, presence, frequency, bias, mask, maskRows))
 
     def unshardCols(self, gathered: Tensor, world: int) -> Tensor:
         """[world*M, Ns] column shards stacked along rows -> the row-major [M, world*Ns] product."""
