@@ -848,11 +848,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   const int rt = pp.rowtiles - 1 - at % pp.rowtiles, unit = at / pp.rowtiles, s = unit / p.H, h = unit - s * p.H;  // (longest first)
   if (tid == 0) {
     tc::mbar_init(s_full, 2);  // the products, and who issued them: the scales of the tile come with it
-    tc::mbar_init(p_full, 256);
+    tc::mbar_init(p_full, 8);  // one arrival a warp here and below: a lane's own would come one after the other
     tc::mbar_init(pv_done, 1);
-    tc::mbar_init(k_full, 256);
-    tc::mbar_init(v_full, 256);
-    tc::mbar_init(code_free, 256);
+    tc::mbar_init(k_full, 8);
+    tc::mbar_init(v_full, 8);
+    tc::mbar_init(code_free, 8);
     tc::mbar_init(code_full, 1);
     tc::mbar_init(code_full + 8, 1);
     tc::fence_barrier_init();
@@ -967,6 +967,10 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
 
   if (warp < 8) {
     const int g = lane >> 2, t = lane & 3;
+    auto arrive = [&](uint32_t b) {
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(b);
+    };
     // a warp's share of tile k: block `quad`, half of its channels
     auto stage = [&](int k) { return smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES + quad * BB; };
     auto keys = [&](int k) {
@@ -1001,7 +1005,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         scl[k & 1][quad][0] = sc.x * kScoreUnit, scl[k & 1][quad][1] = __log2f(wf), scl[k & 1][quad][2] = 1.0f / wf;
       }
       tc::fence_proxy_async_smem();
-      tc::mbar_arrive(k_full);
+      arrive(k_full);
     };
     auto values = [&](int k) {
       const uint8_t *blk = stage(k) + kBlock * HDP;
@@ -1019,8 +1023,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         *(uint4 *)dst = x, *(uint4 *)(dst + 1024) = y;
       }
       tc::fence_proxy_async_smem();
-      tc::mbar_arrive(v_full);
-      tc::mbar_arrive(code_free);
+      arrive(v_full);
+      if (lane == 0) tc::mbar_arrive(code_free);
       if (fetched < nt) {
         if (tid == 0) wait(code_free, k & 1), fetch(fetched);
         fetched++;
@@ -1117,7 +1121,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       }
       tmem_st_wait();
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full);
+      arrive(p_full);
       if (k + 1 < nt) {  // the next tile, while the products run: K is free since the scores came, V when this tile's have run
         keys(k + 1);
         wait(pv_done, k & 1);
