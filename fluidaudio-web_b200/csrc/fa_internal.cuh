@@ -90,7 +90,7 @@ struct fa_kv8 {
   int HDP = 0, nblk = 0;            // width as stored (a form the attention kernels are built for), blocks of a head
   uint8_t *codes = nullptr;         // [S][H][nblk] blocks
   float *tail = nullptr;            // [S][H][2][32][HD]: f32 rows of the block that was written last, keys then values
-  int *tag = nullptr;               // [S][H][2]: which block that is
+  int *tag = nullptr;               // [S][H][2]: the position behind the tail's last row
   int *tickets = nullptr;           // [S][H] arrival counters of the attention's parts, zero between launches
 };
 

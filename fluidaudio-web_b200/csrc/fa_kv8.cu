@@ -23,6 +23,7 @@ struct WriteParams {
   int *tag;
   kv8::Rows rows;
   int H, HD, nblk;
+  int run;  // blocks of a thread block
   int vec;  // rows may be read four values at a time
   int *status;
 };
@@ -89,7 +90,8 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
                                             bool is_last, uint32_t *sw, uint32_t *smax) {
   constexpr int N4 = HDP / 4, ITEMS = WHICH ? (2 * HDP + kThreads - 1) / kThreads * 4 : HDP / 16;
   const int HD = p.HD;
-  const bool kept = held > 0 && *tag == b;  // (read before the barrier in front of its update)
+  // rows of this block that the tail holds; *tag is the position behind its last (read before the barrier in front of its update)
+  const int known = held > 0 && (*tag - 1) >> 5 == b ? *tag - b * kBlock : 0;
   float4 x[ITEMS];
   auto at = [&](int k, int &r, int &d) {  // row and channel of the k-th four values
     if (WHICH == 0) {
@@ -107,7 +109,8 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
     int r, d;
     at(k, r, d);
     x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r >= held && r < rows && d < HD) {
+    if (r >= rows || d >= HD) continue;
+    if (r >= held) {
       const T *q = src + (long long)r * p.ld + d;
       if (p.vec) {
         x[k] = load4(q);
@@ -117,14 +120,7 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
         if (d + 2 < HD) x[k].z = load1(q + 2);
         if (d + 3 < HD) x[k].w = load1(q + 3);
       }
-    }
-  }
-  if (kept) {
-#pragma unroll
-    for (int k = 0; k < ITEMS; k++) {
-      int r, d;
-      at(k, r, d);
-      if (r >= held || d >= HD) continue;
+    } else {  // (asked for before it is known whether the tail is this block's)
       const float *q = tail + r * HD + d;
       if (HD % 4 == 0) {
         x[k] = *(const float4 *)q;
@@ -135,12 +131,15 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
         if (d + 3 < HD) x[k].w = q[3];
       }
     }
-  } else if (held > 0) {
+  }
+  if (held > known) {  // back in an earlier block: its stored values; past rows that nothing wrote: zeros
 #pragma unroll
     for (int k = 0; k < ITEMS; k++) {
       int r, d;
       at(k, r, d);
-      if (r >= held || d >= HD) continue;
+      if (r < known || r >= held || d >= HD) continue;
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (known > 0) continue;
       x[k].x = stored(blk, WHICH, r, d, HDP);
       if (d + 1 < HD) x[k].y = stored(blk, WHICH, r, d + 1, HDP);
       if (d + 2 < HD) x[k].z = stored(blk, WHICH, r, d + 2, HDP);
@@ -183,7 +182,7 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
     for (int k = 0; k < ITEMS; k++) {
       int r, d;
       at(k, r, d);
-      if (r >= rows || (r < held && kept)) continue;
+      if (r >= rows || r < min(held, known)) continue;
       float *q = tail + r * HD + d;
       if (d >= HD) continue;
       if (HD % 4 == 0) {
@@ -195,16 +194,17 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
         if (d + 3 < HD) q[3] = x[k].w;
       }
     }
-    if (threadIdx.x == 0) *tag = b;
+    if (threadIdx.x == 0) *tag = b * kBlock + rows;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * HDP; i += kThreads) ((uint4 *)(blk + (size_t)WHICH * kBlock * HDP))[i] = ((const uint4 *)sw)[i];
   if (threadIdx.x == 0) ((float *)(blk + (size_t)2 * kBlock * HDP))[WHICH] = scale;
 }
 
-// One (stream, head, keys or values): the thread block of x == 0 takes the first and the last block that the rows touch, one
-// after the other, since the first may need the tail that the last one replaces; the others take one block in between.
-// Bound by HBM: 4 bytes in, 1 out.
+// One (stream, head, keys or values) and a run of blocks.  The thread block of x == 0 takes the last block that the rows touch
+// too, behind its own: the first may need the tail that the last one replaces.
+// Bound by HBM, 4 bytes in, 1 out, where rows are many, and then close to what the SMs issue (a run of four blocks shares
+// what a thread block has to find out first); by the latency of a load and two barriers for one row.
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 8 : HDP <= 128 ? 5 : 3) k_kv8_write(const WriteParams p) {
   __shared__ __align__(16) uint32_t sw[8 * HDP];
@@ -220,15 +220,16 @@ __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 8 : HDP <= 128 ? 5 : 3) 
   const size_t unit = (size_t)s * p.H + h;
   float *tail = p.tail + (unit * 2 + which) * kBlock * p.HD;
   const T *src = (const T *)(which ? p.values : p.keys) + ((long long)s * p.rows.T - start) * p.ld + h * p.HD;  // + position * ld
-  const int turns = blockIdx.x == 0 ? 1 + (last > first) : (int)blockIdx.x < last - first;
-  for (int turn = 0; turn < turns; turn++) {
-    const int b = blockIdx.x == 0 ? (turn ? last : first) : first + (int)blockIdx.x, base = b * kBlock;
+  const int b0 = first + (int)blockIdx.x * p.run, b1 = min(last, b0 + p.run);  // the last block is the first thread block's
+  auto one = [&](int b) {
+    const int base = b * kBlock, held = max(0, start - base), rows = min(kBlock, end - base);  // rows from before the call, and in all
     uint8_t *blk = p.codes + (unit * p.nblk + b) * kv8::block_bytes(HDP);
-    const int held = max(0, start - base), rows = min(kBlock, end - base);  // rows from before the call, and in all
     if (which == 0) write_block<T, HDP, 0>(p, src + (long long)base * p.ld, tail, blk, p.tag + unit * 2, b, held, rows, b == last, sw, smax);
     else write_block<T, HDP, 1>(p, src + (long long)base * p.ld, tail, blk, p.tag + unit * 2 + 1, b, held, rows, b == last, sw, smax);
     __syncthreads();
-  }
+  };
+#pragma unroll 1
+  for (int b = b0, left = max(0, b1 - b0) + (blockIdx.x == 0); left > 0; left--, b++) one(left == 1 && blockIdx.x == 0 ? last : b);
 }
 
 template <typename T>
@@ -360,7 +361,9 @@ int fa_kv8_write_rows(fa_ctx *ctx, fa_kv8 *c, const void *k, const void *v, bool
   p.vec = c->HD % 4 == 0 && ld % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & mask) == 0;
   p.status = ctx->dev_status;
   const int touched = pos ? ceil_div(T + kBlock - 1, kBlock) : (n + T - 1) / kBlock - n / kBlock + 1;
-  const dim3 grid(touched > 1 ? touched - 1 : 1, 2 * c->H, c->S);  // (the first thread block takes two)
+  // runs of four while there are four thread blocks for each place on the SMs all the same
+  p.run = (long long)touched * 2 * c->H * c->S >= 128ll * ctx->sm_count ? 4 : 1;
+  const dim3 grid(touched > 1 ? ceil_div(touched - 1, p.run) : 1, 2 * c->H, c->S);
   {
     LaunchScope ls(ctx, "kv8_write");
     if (f16) launch_write<__half>(ctx, p, grid, c->HDP);

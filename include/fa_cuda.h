@@ -278,7 +278,8 @@ int fa_attn_step_append(fa_ctx *ctx, const fa_tensor *qkv, fa_tensor *cache_k, f
  * scale = max|x| / 127 over a block of 32 positions of one head (a block with an infinity or a NaN reads as NaN, one of
  * zeros as zeros).  A block that is not full is coded from its f32 rows again whenever a row joins it, so what is stored
  * depends on the rows alone; a call that goes back to a block before the last one written takes that block's earlier rows at
- * their stored values.  Positions that nothing was written to read as zeros.
+ * their stored values.  Behind the last row of a call its block is empty again; other blocks stay.  Positions that nothing
+ * was written to read as zeros.
  * `pos`, `counts`, `lens`: optional f32 tensors of one whole number per stream that only the device reads; a value outside the
  * cache or the call's rows is clamped and makes the next fa_sync fail with FA_ERR_INVALID. */
 int fa_kv8_create(fa_ctx *ctx, int S, int positions, int H, int HD, fa_kv8 **out);

@@ -183,6 +183,28 @@ def test_going_back_to_an_earlier_block(ctx, cache):
     assert np.array_equal(got(ctx, ctx.kvRead8(c, 0, 5)[0]), stored(x[:5]))
 
 
+@pytest.mark.parametrize("HD", [64, 30])
+def test_places_that_nothing_wrote_are_zeros(ctx, cache, HD):
+    """Rows behind a gap, in a new block, in a block of which the f32 rows are held, and behind a shorter rewrite."""
+    rng = np.random.default_rng(8)
+    x, z = make(rng, 1, 80, HD), np.zeros((6, HD), f32)
+    c = cache(1, 128, 1, HD)
+    write = lambda a, b: ctx.kvWrite8(c, put(ctx, x[a:b]), put(ctx, x[a:b]), a)  # noqa: E731
+    write(0, 32)  # the f32 rows of a full block are held
+    write(32, 34)
+    write(40, 41)  # 34..39 are nobody's, and not rows 2..7 of the block before
+    for t in ctx.kvRead8(c, 32, 9):
+        assert np.array_equal(got(ctx, t), stored(np.concatenate([x[32:34], z, x[40:41]])))
+    write(34, 35)  # ends the block behind it
+    write(36, 37)
+    for t in ctx.kvRead8(c, 32, 9):
+        assert np.array_equal(got(ctx, t), stored(np.concatenate([x[32:35], z[:1], x[36:37], z[:4]])))
+    write(69, 72)  # a block without its first rows
+    for t in ctx.kvRead8(c, 64, 8):
+        assert np.array_equal(got(ctx, t), stored(np.concatenate([z[:5], x[69:72]])))
+    assert np.array_equal(got(ctx, ctx.kvRead8(c, 0, 32)[0]), stored(x[:32]))
+
+
 def test_streams_at_positions_of_their_own(ctx, cache):
     S, H, HD, T = 5, 2, 64, 40
     rng = np.random.default_rng(4)
