@@ -475,12 +475,15 @@ __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const Attn
   if (threadIdx.x < 2) open_unit[threadIdx.x] = -1;
   tc::fence_barrier_init();
   __syncthreads();
-  fa_grid_dep_sync();
-
   Sight sight;
   bool bad;
   const int each = p.H * p.rowgroups;  // units of a stream
   const bool ragged = p.lens || p.rows.pos || p.rows.counts;
+  // Where the launch in front is the one that writes this call's rows (which lets go of this one only when all before it has
+  // ended), the first blocks that it does not touch are fetched while it runs.
+  const int ready = p.causal && !ragged ? p.rows.n / kBlock : 0;
+  if (ready) fa_grid_dep_launch();
+  else fa_grid_dep_sync();
   const int shares = (int)gridDim.x * kWarps, mine = (int)blockIdx.x * kWarps + warp;
   int total = 0, per, unit = 0, b0 = 0, base = 0;  // places, a share, its first unit, first block in that, the unit's place in the list
   if (!ragged) {
@@ -543,14 +546,18 @@ __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const Attn
   } else {
     base = f1;
   }
-  if (base < f1) {
+  if (base >= f1) {
+    if (ready) fa_grid_dep_wait();
+  } else {
     place(unit, s, h, row0);
     sight.of(p, s, bad);
     const uint32_t slots = smem_u32(ring) + warp * (NST * BB), bars = smem_u32(&full[warp][0]);
     // the next block to fetch
     int pu = unit, pbase = base, pnb = sight.blocks(), pleft = min(pnb, f1 - pbase) - b0, pst = 0;
     const uint8_t *psrc = p.codes + ((size_t)(pu / p.rowgroups) * p.nblk + b0) * BB;
-    auto fetch = [&]() {  // (all lanes keep the place, one issues)
+    int pb = b0;  // (kept for the first fetches)
+    bool waited = ready == 0;
+    auto fetch = [&](bool first) {  // (all lanes keep the place, one issues)
       if (pleft == 0) {
         pbase += pnb + kTurn, pu++;
         if (pbase >= f1) {
@@ -565,7 +572,9 @@ __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const Attn
         }
         pleft = min(pnb, f1 - pbase);
         psrc = p.codes + (size_t)(pu / p.rowgroups) * p.nblk * BB;
+        pb = 0;
       }
+      if (first && !waited && pb++ >= ready) fa_grid_dep_wait(), waited = true;
       if (lane == 0) {
         tc::mbar_expect_tx(bars + 8 * pst, BB);
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(slots + pst * BB),
@@ -576,7 +585,8 @@ __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const Attn
       if (++pst == NST) pst = 0;
     };
 #pragma unroll 1
-    for (int k = 0; k < NST; k++) fetch();
+    for (int k = 0; k < NST; k++) fetch(true);
+    if (!waited) fa_grid_dep_wait();
 
     int st = 0, parity = 0;
 #pragma unroll 1
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const Attn
         ok = __all_sync(0xffffffffu, tc::mbar_wait(bars + 8 * st, parity, p.wait_limit)) && ok;
         acc.block(ring + (warp * NST + st) * BB, b * kBlock, (b + 1) * kBlock <= least, lane);
         __syncwarp();
-        fetch();
+        fetch(false);
         if (++st == NST) st = 0, parity ^= 1;
       }
       const int slot = 2 * warp + (b0 == 0);  // the part in front of all others, or behind

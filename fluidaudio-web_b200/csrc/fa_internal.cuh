@@ -257,9 +257,11 @@ struct LaunchScope {
 // fa_grid_dep_sync() before it reads or writes anything its predecessors touch: the call first lets the NEXT
 // grid in the stream be scheduled early in turn, then waits until every earlier grid has completed and its
 // writes are visible.  Without the attribute (option "pdl" = 0, or a plain <<<>>> launch) the call is a no-op.
+__device__ __forceinline__ void fa_grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void fa_grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void fa_grid_dep_sync() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  fa_grid_dep_launch();
+  fa_grid_dep_wait();
 }
 
 template <typename... KArgs, typename... Args>

@@ -209,7 +209,8 @@ template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 8 : HDP <= 128 ? 5 : 3) k_kv8_write(const WriteParams p) {
   __shared__ __align__(16) uint32_t sw[8 * HDP];
   __shared__ uint32_t smax[kThreads / 32];
-  fa_grid_dep_sync();
+  fa_grid_dep_wait();
+  fa_grid_dep_launch();  // (after the wait: what follows may then read what lies further back without a wait of its own)
   const int h = blockIdx.y >> 1, which = blockIdx.y & 1, s = blockIdx.z;
   int start, count;
   bool bad;

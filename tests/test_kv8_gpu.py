@@ -379,6 +379,34 @@ def test_recorded_and_replayed(ctx, cache):
     batch.free()
 
 
+@pytest.mark.parametrize("S,H,n", [(1, 20, 447), (48, 12, 200), (3, 4, 31)])
+def test_tokens_in_a_row_without_a_pause(ctx, cache, S, H, n):
+    """Each token reads what the call before it wrote: one recording against calls that wait for one another."""
+    rng = np.random.default_rng(23)
+    steps, w = 6, H * 64
+    k, v = make(rng, S, n, w), make(rng, S, n, w)
+    xs = [put(ctx, make(rng, S, 1, 3 * w, 0.3)) for _ in range(steps)]
+    tk, tv = put(ctx, k), put(ctx, v)
+
+    def run(c, pause):
+        ctx.kvWrite8(c, tk, tv)
+        out = []
+        for i in range(steps):
+            out.append(ctx.attnAppendKv8(xs[i], c, H, n + i))
+            if pause:
+                ctx.sync()
+        return out
+
+    c = cache(S, n + steps, H, 64)
+    want = [got(ctx, t) for t in run(c, True)]
+    graph, outs = ctx.recordBatch(lambda: run(c, False))
+    for _ in range(3):
+        graph.launch()
+        for t, y in zip(outs, want):
+            assert np.array_equal(got(ctx, t), y)
+    graph.free()
+
+
 def test_lengths_outside_are_reported(ctx, cache, pkg):
     S, H, HD, n = 2, 1, 64, 40
     rng = np.random.default_rng(11)
