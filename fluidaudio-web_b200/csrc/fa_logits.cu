@@ -14,12 +14,17 @@
 // is rounded by itself, so the values are those of the formulas in f32 whatever the split.
 // Bound by HBM where rows are many (4 bytes in, 4 out; the counters stay on the chip), by the latency of two cluster barriers
 // and one round of loads where they are few.
+#include <algorithm>
+#include <type_traits>
+
 #include "fa_internal.cuh"
 
 namespace {
 
-constexpr int kThreads = 512, kMaxCluster = 8, kBatch = 4;
-constexpr int kSlice = 49152;  // tokens that a thread block counts at a time: 192 KB
+constexpr int kMaxCluster = 8;
+constexpr int kBatch = 4;            // tokens of a thread at a time, and as many on their way
+constexpr int kCountBytes = 196608;  // of a thread block's counts at a time
+constexpr int kFew = 512, kMany = 256;  // threads of a block, see `rules`
 
 struct LogitParams {
   const float *x;
@@ -63,10 +68,14 @@ __device__ __forceinline__ void to_l2(const float *p, int n) {
   if (n > 0 && to > from) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from)) : "memory");
 }
 
-// PICK: the best token instead of the logits; HISTORY, BIAS, MASK: which rules there are
-template <bool PICK, bool HISTORY, bool BIAS, bool MASK>
-__global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
-  extern __shared__ uint32_t cnt[];  // one slice's counts
+// PICK: the best token instead of the logits; HISTORY, BIAS, MASK: which rules there are.  HISTORY 1 counts in 16 bits (fewer
+// than 65536 tokens), 2 in 32.
+template <int kThreads, bool PICK, int HISTORY, bool BIAS, bool MASK>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_adjust(const LogitParams p) {
+  using Count = std::conditional_t<HISTORY == 1, uint16_t, uint32_t>;
+  constexpr int kSlice = kCountBytes / (int)sizeof(Count);
+  extern __shared__ uint32_t words[];
+  const Count *cnt = (const Count *)words;  // one slice's counts
   __shared__ float bv[kThreads / 32];
   __shared__ int bi[kThreads / 32];
   __shared__ float cv;  // this block's best, read by rank 0
@@ -125,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
     };
     load();
     if (HISTORY) {
-      for (int i = threadIdx.x; i < min(width, kSlice); i += kThreads) cnt[i] = 0;
+      for (int i = threadIdx.x; i < min(width, kSlice) / (4 / (int)sizeof(Count)); i += kThreads) words[i] = 0;
       cluster_sync();
       const int i0 = (int)((long long)p.n * rank / nc), i1 = (int)((long long)p.n * (rank + 1) / nc);
       for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {
@@ -133,12 +142,13 @@ __global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
         if (!(f >= 0.0f && f < (float)p.V)) continue;
         const int token = (int)f, owner = token / width, c = token - owner * width - off;
         if (c >= 0 && c < kSlice)
-          asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], 1;" ::"r"(in_block(cnt + c, owner)) : "memory");
+          asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(in_block(words + (HISTORY == 1 ? c >> 1 : c), owner)),
+                       "r"(HISTORY == 1 && (c & 1) ? 65536u : 1u)
+                       : "memory");
       }
       cluster_sync();
     }
-    auto step = [&](int u) {
-      float y = x[u];
+    auto step = [&](int u, float y, float add, uint32_t word) {
       if (HISTORY) {
         const uint32_t c = cnt[k + u * kThreads];
         if (c) {
@@ -146,8 +156,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
           y = __fsub_rn(__fsub_rn(y, __fmul_rn((float)c, p.frequency)), p.presence);
         }
       }
-      if (BIAS) y = __fadd_rn(y, bb[u]);
-      const bool allowed = !MASK || (w[u] >> (threadIdx.x & 31) & 1u);
+      if (BIAS) y = __fadd_rn(y, add);
+      const bool allowed = !MASK || (word >> (threadIdx.x & 31) & 1u);
       if (PICK) {
         if (allowed && (y > best || (y == best && a + k + u * kThreads < at))) best = y, at = a + k + u * kThreads;  // (a NaN never wins)
       } else {
@@ -155,12 +165,22 @@ __global__ void __launch_bounds__(kThreads, 3) k_adjust(const LogitParams p) {
       }
     };
     while (left > 0) {
+      float y[kBatch], add[BIAS ? kBatch : 1];
+      uint32_t word[MASK ? kBatch : 1];
+#pragma unroll
+      for (int u = 0; u < kBatch; u++) {
+        y[u] = x[u];
+        if (BIAS) add[u] = bb[u];
+        if (MASK) word[u] = w[u];
+      }
+      const int now = left;
+      left -= kBatch * kThreads;
+      if (left > 0) load();
 #pragma unroll
       for (int u = 0; u < kBatch; u++)
-        if (u * kThreads < left) step(u);
-      left -= kBatch * kThreads, k += kBatch * kThreads;
+        if (u * kThreads < now) step(u, y[u], BIAS ? add[BIAS ? u : 0] : 0.0f, MASK ? word[MASK ? u : 0] : 0u);
+      k += kBatch * kThreads;
       if (!PICK) po += kBatch * kThreads;
-      if (left > 0) load();
     }
     if (HISTORY && off + kSlice < width) cluster_sync();  // (the counts are read)
   }
@@ -249,24 +269,33 @@ int rules(fa_ctx *ctx, const fa_tensor *x, int ncols, const fa_logit_rules *r, b
   FA_TRY(fa_tensor_new(ctx, p.S, pick ? 2 : p.V, FA_F32, true, &y));
   if (p.S) {
     p.out = (float *)y->dptr, p.status = ctx->dev_status;
+    // Blocks of a row: as many as one wave of two blocks an SM takes, and so many that a block's tokens are at most 16640.  The
+    // two shapes of a block, us, 512 threads (two an SM) / 256 (four): one row of 51866 tokens, pick 6.4 / 7.4; 64 rows 10.3 /
+    // 14.7; 256 rows of 131075, values 127 / 114, pick 148 / 121.  More threads an SM of either shape are slower for many rows
+    // (256 x 6: 145): the loads of one batch wait behind the others'.
     int nc = 1;
-    while (nc < kMaxCluster && p.V > nc * 2048 && (p.S * nc * 2 <= 3 * ctx->sm_count || p.V > nc * 16640)) nc *= 2;
+    while (nc < kMaxCluster && p.V > nc * 2048 && (p.S * nc <= ctx->sm_count || p.V > nc * 16640)) nc *= 2;
     const int width = (int)round_up(ceil_div(p.V, nc), 32);
-    const size_t smem = p.history ? (size_t)4 * (width < kSlice ? width : kSlice) : 0;
+    const int counts = !p.history ? 0 : p.n < 65536 ? 1 : 2;
+    const bool few = (long long)p.S * nc <= 2 * ctx->sm_count || counts == 2;
+    const size_t smem = counts ? std::min<size_t>((size_t)width * (counts == 1 ? 2 : 4), kCountBytes) : 0;
     using Kernel = void (*)(LogitParams);
-    static const Kernel kernels[2][8] = {
-        {k_adjust<false, false, false, false>, k_adjust<false, false, false, true>, k_adjust<false, false, true, false>, k_adjust<false, false, true, true>,
-         k_adjust<false, true, false, false>, k_adjust<false, true, false, true>, k_adjust<false, true, true, false>, k_adjust<false, true, true, true>},
-        {k_adjust<true, false, false, false>, k_adjust<true, false, false, true>, k_adjust<true, false, true, false>, k_adjust<true, false, true, true>,
-         k_adjust<true, true, false, false>, k_adjust<true, true, false, true>, k_adjust<true, true, true, false>, k_adjust<true, true, true, true>}};
-    static SmemLimit limit[2][8];
-    const int which = (p.history ? 4 : 0) + (p.bias ? 2 : 0) + (p.mask ? 1 : 0);
-    const Kernel kernel = kernels[pick][which];
-    cudaError_t e = p.history ? limit[pick][which].raise(ctx, kernel, kSlice * 4) : cudaSuccess;
+#define FORMS(THREADS, PICK, HISTORY)                                                                        \
+  {k_adjust<THREADS, PICK, HISTORY, false, false>, k_adjust<THREADS, PICK, HISTORY, false, true>,            \
+   k_adjust<THREADS, PICK, HISTORY, true, false>, k_adjust<THREADS, PICK, HISTORY, true, true>}
+#define ROWS(PICK) {FORMS(kMany, PICK, 0), FORMS(kMany, PICK, 1), FORMS(kFew, PICK, 0), FORMS(kFew, PICK, 1), FORMS(kFew, PICK, 2)}
+    static const Kernel kernels[2][5][4] = {ROWS(false), ROWS(true)};
+#undef ROWS
+#undef FORMS
+    static SmemLimit limit[2][5][4];
+    const int form = few ? 2 + counts : counts;
+    const int which = (p.bias ? 2 : 0) + (p.mask ? 1 : 0);
+    const Kernel kernel = kernels[pick][form][which];
+    cudaError_t e = p.history ? limit[pick][form][which].raise(ctx, kernel, kCountBytes) : cudaSuccess;
     if (e == cudaSuccess) {
       LaunchScope ls(ctx, pick ? "pick_adjusted" : "adjust_logits");
       cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3((unsigned)(p.S * nc)), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
+      cfg.gridDim = dim3((unsigned)(p.S * nc)), cfg.blockDim = dim3(few ? kFew : kMany), cfg.dynamicSmemBytes = smem, cfg.stream = ctx->stream;
       cudaLaunchAttribute attr[2];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = nc, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;

@@ -142,6 +142,17 @@ def test_one_token_many_times(ctx):
     assert y[0, 7] == 1 - n and np.array_equal(np.delete(y, 7), np.ones(49, f32))
 
 
+@pytest.mark.parametrize("S", [1, 400])
+@pytest.mark.parametrize("n", [65535, 65536])
+def test_counts_at_the_end_of_16_bits(ctx, S, n):
+    x = np.ones((S, 50), f32)
+    hist = np.full((n, 1), 6) + np.arange(S) % 2  # the even one of a pair, or the odd one
+    y = got(ctx, ctx.adjustLogits(put(ctx, x), history=put(ctx, hist), n=n, frequency=1.0))
+    want = x.copy()
+    want[np.arange(S), 6 + np.arange(S) % 2] = 1 - n
+    assert np.array_equal(y, want)
+
+
 def test_recorded_with_a_growing_history(ctx):
     """A decode of a few tokens, picks written into the history on the device, recorded once and replayed."""
     S, V, n = 3, 501, 6
