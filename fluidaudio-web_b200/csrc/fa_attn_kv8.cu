@@ -408,6 +408,8 @@ struct ManyRows {
   }
 };
 
+// Blocks on their way per warp: 4 KB each at 64 channels, three thread blocks an SM, so 192 KB an SM.  (More of them, or more
+// warps, gave nothing; blocks a multiple of 128 bytes apart neither.)
 template <int HDP>
 __host__ __device__ constexpr int stages() { return HDP <= 32 ? 8 : HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1; }
 // rings, then two results of each warp, `rows` rows each
@@ -458,6 +460,12 @@ struct Joined {
 // another's blocks.  A unit inside a share is finished by its warp.  The others meet first in the thread block, whose warps'
 // shares are neighbours, then, where a unit lies in several thread blocks, in the one that takes the last ticket; parts are
 // joined in the list's order (nothing waits, and the result does not depend on who comes last).
+//
+// Bound by HBM where blocks are many: 64 streams, one token, 20 heads of 64 over 1500 positions (247 MB) 51.7 us = 4.8 TB/s; 4
+// streams, 32 query heads on 8 of 128, 65551 positions (538 MB) 98 us = 5.5 TB/s; by a chain of latencies where they are few
+// (one stream of the former 8.9 us).  What is left of the former is that the SMs stream at different rates, so that equal shares
+// end 15 % apart.  Shares that warps claim one after the other even that out and cost more, in starts, results and joins, than
+// they give (58 to 80 us by their size), as do two or three thread blocks a place on the GPU (58, 64).
 template <int HDP, class Acc>
 __global__ void __launch_bounds__(kThreads, Acc::RESIDENT) k_attn_kv8(const AttnParams p) {
   constexpr int BB = (int)kv8::block_bytes(HDP), NST = stages<HDP>(), ROWS = Acc::ROWS, PITCH = Acc::PITCH, NK = HDP / 32;
@@ -778,6 +786,9 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 //
 // What bounds it: the softmax warps (about 6 instructions an element and one exponential, 16 a clock and SM) and the products,
 // 2 x 128 x 128 x HD x 2 x 2 a tile, cost about the same; two thread blocks an SM overlap them where shared memory allows.
+// A tile costs a thread block about 5900 cycles at two an SM, its start and end 20000.  8 streams of 224 queries, 20 heads of 64
+// over up to 1500 positions of different lengths: 56 us; 16 streams' prompts of 224 over themselves: write and attention 61 us.
+// Separate warps for the softmax and the conversion took 70 us in place of 55, runs of four to eight tiles 72 to 80.
 // From this many rows of a unit on.  Measured, us, groups of 16 rows / this kernel, 16 streams of 20 heads of 64 over 1500
 // positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.
 constexpr int kPromptRows = 49;
