@@ -332,10 +332,15 @@ def cross_kv_streams(ctx, dec, encs, cache: Optional[str] = None, S: int = 0, le
         v = ctx.pin(_mm(ctx, enc_all, w["cvw"], bias=w["cvb"]))
         if cache:
             n = enc_all.rows // S
-            c = ctx.kvWrite8(ctx.kvCache8(S, n, cfg["NH"], cfg["HD"]), k, v, counts=lens)
-            ctx.freeTensor(k)
-            ctx.freeTensor(v)
-            out.append(dict(cache=c, n=n, lens=lens))
+            try:
+                out.append(dict(cache=ctx.kvCache8(S, n, cfg["NH"], cfg["HD"]), n=n, lens=lens))
+                ctx.kvWrite8(out[-1]["cache"], k, v, counts=lens)
+            except Exception:
+                free_caches(ctx, out)
+                raise
+            finally:
+                ctx.freeTensor(k)
+                ctx.freeTensor(v)
         else:
             out.append(dict(k=k, v=v))
     return out
@@ -350,7 +355,14 @@ def free_caches(ctx, kv: Optional[list] = None, st: Optional[dict] = None) -> No
 def decode_init_streams(ctx, dec, S: int, maxLen: int = 448, cache: Optional[str] = None) -> dict:
     D = dec["cfg"]["D"]
     if cache == "int8":
-        return dict(n=0, S=S, maxLen=maxLen, self8=[ctx.kvCache8(S, maxLen, dec["cfg"]["NH"], dec["cfg"]["HD"]) for _ in dec["layers"]])
+        st = dict(n=0, S=S, maxLen=maxLen, self8=[])
+        try:
+            for _ in dec["layers"]:
+                st["self8"].append(ctx.kvCache8(S, maxLen, dec["cfg"]["NH"], dec["cfg"]["HD"]))
+        except Exception:
+            free_caches(ctx, st=st)
+            raise
+        return st
     if cache is not None:
         raise ValueError(f"decode_init_streams: cache {cache!r}")
     return dict(n=0, S=S, maxLen=maxLen, selfK=[ctx.pin(ctx.alloc(maxLen, S * D)) for _ in dec["layers"]],
@@ -433,9 +445,9 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
     S = len(encs)
     own_kv, own_st = kv is None, st is None
     kv = cross_kv_streams(ctx, dec, encs, cache, lens=lens) if own_kv else kv
-    st = decode_init_streams(ctx, dec, S, len(prefix) + n_tokens, cache) if own_st else st
-    st["n"] = st["picked"] = 0
     try:
+        st = decode_init_streams(ctx, dec, S, len(prefix) + n_tokens, cache) if own_st else st
+        st["n"] = st["picked"] = 0
         nxt = None
         if "self8" in st:
             nxt, _ = prefill_streams(ctx, dec, kv, st, np.tile(np.asarray(prefix, np.int64), (S, 1)), rules=rules)
@@ -450,7 +462,7 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
         return out
     finally:
         free_caches(ctx, kv if own_kv else None, st if own_st else None)
-        if own_st and "hist" in st:
+        if own_st and st and "hist" in st:
             ctx.freeTensor(st["hist"])
 
 

@@ -209,3 +209,29 @@ def test_what_the_engine_refuses(ctx, pkg):
     assert wd.decode_next_streams(ctx, dec, kv8, st8, [1, 2], rules=dict(mask=none))[0].tolist() == [-1, -1]
     wd.free_caches(ctx, kv8, st8)
     wd.free_caches(ctx, kv8, st8)  # twice is no error: the handles are gone
+
+
+def test_caches_go_back_when_one_cannot_be_made(ctx, pkg, monkeypatch):
+    wd, cfg, dec, states = _setup(ctx, 2)
+    live, make, free = set(), ctx.kvCache8, ctx.freeKvCache8
+
+    def limited(*a):
+        if len(live) == limit:
+            raise pkg.CudaError(-2, "out of memory")
+        c = make(*a)
+        live.add(id(c))
+        return c
+
+    def back(c):
+        live.discard(id(c))
+        free(c)
+
+    monkeypatch.setattr(ctx, "kvCache8", limited)
+    monkeypatch.setattr(ctx, "freeKvCache8", back)
+    layers = len(dec["layers"])
+    for limit, call in ((1, lambda: wd.cross_kv_streams(ctx, dec, states, "int8", S=2)), (1, lambda: wd.decode_init_streams(ctx, dec, 2, 10, "int8")),
+                        (layers + 1, lambda: wd.greedy_decode_streams(ctx, dec, list(two), [1, 2], 3, cache="int8"))):
+        two = [ctx.upload(np.ones((cfg["Tenc"], cfg["D"]), f32), cfg["Tenc"], cfg["D"]) for _ in range(2)]
+        with pytest.raises(pkg.CudaError, match="out of memory"):
+            call()
+        assert not live
