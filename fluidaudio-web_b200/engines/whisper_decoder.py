@@ -413,6 +413,8 @@ def prefill_streams(ctx, dec, kv, st, tokens, want_logits: bool = False, rules: 
         raise ValueError("prefill_streams: a token id below 0 (a stream whose rules allowed no token)")
     if rules is not None and want_logits:
         raise ValueError("prefill_streams: rules are for the pick on the device")
+    if n + T > dec["pos"].shape[0]:  # (a slice that ends early would be broadcast over the tokens)
+        raise IndexError(f"prefill_streams: positions {n}..{n + T - 1} of a table of {dec['pos'].shape[0]}")
     emb = dec["embed"][tokens] + dec["pos"][n:n + T][None, :, :]
     x = ctx.upload(np.ascontiguousarray(emb, dtype=f32), S * T, D)
     arena = ctx.pushArena()

@@ -1,0 +1,32 @@
+"""What the lock-step decoder refuses before anything is computed, on the CPU oracle."""
+import numpy as np
+import pytest
+
+from oracle.wasm_oracle import WasmOracle
+
+
+@pytest.fixture
+def setup(pkg):
+    from fluidaudio_web_b200.engines import synth, whisper_decoder as wd
+
+    cfg, ctx, S = synth.TINY_DEC, WasmOracle(), 2
+    dec = wd.load_decoder(ctx, synth.decoder_weights(cfg), cfg["NH"])
+    encs = [ctx.upload(e, cfg["Tenc"], cfg["D"]) for e in synth.encoder_states(cfg, S)]
+    return wd, ctx, dec, encs, S
+
+
+def test_tokens_behind_the_position_table(setup):
+    """A cache may be longer than the table: the last place of the table works, one behind it is refused and nothing moves."""
+    wd, ctx, dec, encs, S = setup
+    table = dec["pos"].shape[0]
+    kv, st = wd.cross_kv_streams(ctx, dec, encs), wd.decode_init_streams(ctx, dec, S, table + 8)
+    st["n"] = table - 1
+    wd.decode_next_streams(ctx, dec, kv, st, [1] * S)
+    assert st["n"] == table
+    with pytest.raises(IndexError):
+        wd.decode_next_streams(ctx, dec, kv, st, [1] * S)
+    assert st["n"] == table
+    # prompts: with one row of the table left it would stand for all tokens
+    for n, T in ((table - 1, 2), (table - 1, 5), (table, 2), (0, table + 1)):
+        with pytest.raises(IndexError):
+            wd.prefill_streams(ctx, dec, kv, dict(n=n, S=S, self8=[]), np.ones((S, T)))
