@@ -780,9 +780,12 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 // S in TMEM, 32 positions at a time (16 columns of values, 16 of residues), and is the TMEM operand of the second product.
 // The next tile's K is made while a tile's P V runs and its V while its own scores are computed.
 //
-// Weights are exp2(s - ref) times the block's values' scale over the largest scale of the range, times 2^kUpP: whole f16 range
-// for what counts, and the accumulator needs no scale of its own per block.  `ref` is a row's maximum when it was last moved:
-// it moves, and the accumulator is rescaled, only when a tile's maximum is more than 2^kSlack above it.
+// A row of P holds the weights times their blocks' value scales, relative to the largest such product that this row has in this
+// tile and times 2^kUpP, so that the whole f16 range is for what counts to the row, and the accumulator needs no scale per block.
+// What other rows see, or blocks that a row gives no weight to, however large their values, is not in it.  A tile's result
+// joins the running one, which has a reference of its own and lies in TMEM beside it.  The sum of the weights alone is kept
+// relative to the largest score; it takes the scales out of the sums of products again, a factor for each block.  References are whole
+// powers of two: what moves between them is not rounded.
 //
 // What bounds it: the softmax warps (about 6 instructions an element and one exponential, 16 a clock and SM) and the products,
 // 2 x 128 x 128 x HD x 2 x 2 a tile, cost about the same; two thread blocks an SM overlap them where shared memory allows.
@@ -792,7 +795,9 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 // From this many rows of a unit on.  Measured, us, groups of 16 rows / this kernel, 16 streams of 20 heads of 64 over 1500
 // positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.
 constexpr int kPromptRows = 49;
-constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6, kSlack = 8;
+constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6;
+// A block's products are at least 2^-kFar of the row's largest ones (as f16 that is 0 all the same): its sum of weights needs them.
+constexpr float kFar = 80.0f;
 
 template <int HDP>
 struct PromptSmem {
@@ -854,9 +859,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   __shared__ __align__(8) uint64_t bar[8];  // see the names below
-  __shared__ float tops[2][2][kTile];        // row maxima of the two halves; their sums of weights in the end
-  __shared__ float scl[2][4][4];            // a tile's scales: keys, in units of log 2; values over the largest, log and reciprocal
-  __shared__ float svmax_of[kPromptThreads / 32];
+  __shared__ float tops[2][2][kTile];        // row maxima of the two halves; their sums of weights and maxima in the end
+  __shared__ float scl[2][4][4];            // a tile's scales: keys, in units of log 2; values as 2^[1] * 2^[2], and 2^-[2]
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const uint32_t s_full = smem_u32(&bar[0]), p_full = smem_u32(&bar[1]), pv_done = smem_u32(&bar[2]), k_full = smem_u32(&bar[3]),
@@ -896,7 +900,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   const int t0 = split * pp.per, t1 = min((most + kTile - 1) / kTile, t0 + pp.per), nt = max(0, t1 - t0);
   const uint8_t *codes = p.codes + (size_t)unit * p.nblk * BB;
 
-  // everything that is read first is asked for together: the codes of two tiles, the query rows, the values' scales
+  // everything that is read first is asked for together: the codes of two tiles, the query rows
   auto fetch = [&](int k) {  // tile k of this range into stage k & 1
     const int b = (t0 + k) * 4, n = min(4, p.nblk - b);
     const uint32_t bytes = (uint32_t)n * BB, dst = smem_u32(smem + Smem::STAGE + (k & 1) * Smem::STAGE_BYTES), on = code_full + 8 * (k & 1);
@@ -936,11 +940,6 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       }
     }
   }
-  float svmax = 0.0f;  // the largest scale of the range's values
-  for (int b = t0 * 4 + tid; b < min(t1 * 4, (most + kBlock - 1) / kBlock); b += kPromptThreads) {
-    const float sv = *(const float *)(codes + (size_t)b * BB + 2 * kBlock * HDP + 4);
-    if (sv < INFINITY) svmax = fmaxf(svmax, sv);
-  }
   // queries scaled and split as in load_row
   if (warp < 8) {
 #pragma unroll
@@ -964,18 +963,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
     }
     tc::fence_proxy_async_smem();
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) svmax = fmaxf(svmax, __shfl_xor_sync(0xffffffffu, svmax, o));
-  if (lane == 0) svmax_of[warp] = svmax;
   const int quad = warp & 3, half = warp >> 2, local = quad * 32 + lane, row = row_a + local;
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_slot, tS = tmem, tO = tmem + 128, tSum = tO + HDP;
-  svmax = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kPromptThreads / 32; w++) svmax = fmaxf(svmax, svmax_of[w]);
-  if (!(svmax > 0.0f)) svmax = 1.0f;
   const float qs = tops[0][0][local];
   __syncthreads();  // (the array's next use)
   // Where a wait runs out a thread goes on without waiting for anything: every loop ends, every barrier gets its arrivals, and
@@ -984,7 +976,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   auto wait = [&](uint32_t b, uint32_t parity) {
     if (ok) ok = tc::mbar_wait(b, parity, p.wait_limit);
   };
-  float m = -INFINITY, l = 0.0f;
+  // this thread's half of the row: reference and sum of its weights; both halves: references of the running result, of a tile's
+  float m = -INFINITY, l = 0.0f, run_ref = -INFINITY, tile_ref = -INFINITY;
 
   if (warp < 8) {
     const int g = lane >> 2, t = lane & 3;
@@ -1020,10 +1013,13 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       if (half == 0 && lane == 0) {
         const bool there = (t0 + k) * 4 + quad < p.nblk;
         const float2 sc = there ? *(const float2 *)(blk + 2 * kBlock * HDP) : make_float2(0.f, 0.f);
-        // a scale of 0 stands with codes of 0, one of 2^-60 of the largest counts for nothing: both may be any other
-        const float v = sc.y / svmax;
-        const float wf = (v < 8.7e-19f ? 8.7e-19f : v) * (float)(1 << kUpP);
-        scl[k & 1][quad][0] = sc.x * kScoreUnit, scl[k & 1][quad][1] = __log2f(wf), scl[k & 1][quad][2] = 1.0f / wf;
+        // sc.y = 2^e * f, f in [1, 2).  A scale of 0 stands with codes of 0, so it may be any: 2^-200 is below all others.
+        const bool small = sc.y < 1e-30f;
+        const uint32_t bits = __float_as_uint(small ? sc.y * 0x1p64f : sc.y);
+        const float f = sc.y < INFINITY ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : __int_as_float(0x7fc00000);
+        scl[k & 1][quad][0] = sc.x * kScoreUnit;
+        scl[k & 1][quad][1] = sc.y > 0.0f ? (float)((int)(bits >> 23) - (small ? 191 : 127)) : -200.0f;
+        scl[k & 1][quad][2] = log2f(f), scl[k & 1][quad][3] = 1.0f / f;
       }
       tc::fence_proxy_async_smem();
       arrive(k_full);
@@ -1053,10 +1049,12 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
     };
     const int lim = row < nrows ? sight.limit(row / p.G) : 0;
     const uint32_t mine = (uint32_t)(quad * 32) << 16;
-    // what the tile before gave joins the running result, and both go to the new reference: the tensor cores cut off what an f32
-    // cannot hold, so a sum that ran on over many tiles would shrink; within a tile the residues go first
-    auto sum_up = [&](bool more, float f) {
-      const uint64_t f2 = pair(f, f);
+    // what the tile before gave joins the running result at the larger of the two references: the tensor cores cut off what an
+    // f32 cannot hold, so a sum that ran on over many tiles would shrink; within a tile the residues go first
+    auto sum_up = [&](bool more) {
+      const float next = fmaxf(run_ref, tile_ref), f = rescale(tile_ref, next), old = rescale(run_ref, next);
+      const uint64_t f2 = pair(f, f), old2 = pair(old, old);
+      run_ref = next;
 #pragma unroll 1
       for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
         uint32_t x[16], y[16];
@@ -1065,9 +1063,9 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         tc::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          uint64_t v = pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          if (more) v = add2(v, pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])));
-          const float2 r = unpair(mul2(v, f2));
+          uint64_t v = mul2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2);
+          if (more) v = fma2(pair(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), old2, v);
+          const float2 r = unpair(v);
           x[e] = __float_as_uint(r.x), x[e + 1] = __float_as_uint(r.y);
         }
         tmem_st16(tSum + mine + c, x);
@@ -1079,7 +1077,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       __syncwarp();
       tc::tc_fence_after();
       const int seen = lim - (t0 + k) * kTile - 64 * half;  // of this thread's 64 positions
-      float top = -INFINITY;
+      float top0 = -INFINITY, top1 = -INFINITY;  // of the two blocks
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         float v[32];
@@ -1093,18 +1091,20 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
 #pragma unroll
           for (int e = 0; e < 32; e++) t = e < n ? fmaxf(t, v[e]) : t;
         }
-        if (n > 0) top = fmaxf(top, t * (scl[k & 1][2 * half + c][0] * qs));
+        t = n > 0 ? fmaxf(-INFINITY, t * (scl[k & 1][2 * half + c][0] * qs)) : -INFINITY;  // (NaN: no maximum)
+        if (c == 0) top0 = t;
+        else top1 = t;
       }
-      // the row's maximum: the other half's too
-      tops[k & 1][half][local] = top;
+      // the row's largest product of a weight and a scale, the other half's too
+      float most_of = fmaxf(top0 + scl[k & 1][2 * half][1], top1 + scl[k & 1][2 * half + 1][1]);
+      tops[k & 1][half][local] = most_of;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-      top = fmaxf(top, tops[k & 1][1 - half][local]);
-      // a new reference where the maximum has moved far: what was summed so far is rescaled
-      const bool move = top > m + kSlack || (m == -INFINITY && top > -INFINITY);
-      const float old = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-      if (move) m = top, l *= old;
-      if (k > 0) sum_up(k > 1, old);
-      const float ref = m == -INFINITY ? 0.0f : m;
+      most_of = floorf(fmaxf(most_of, tops[k & 1][1 - half][local]));
+      if (k > 0) sum_up(k > 1);
+      tile_ref = most_of;
+      const float ref = tile_ref == -INFINITY ? 0.0f : tile_ref, next = fmaxf(m, floorf(fmaxf(top0, top1)));
+      l *= rescale(m, next);
+      m = next;
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         float v[32];
@@ -1115,7 +1115,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         const float *sc = scl[k & 1][2 * half + c];
         const float f = sc[0] * qs;
         // weights with the values' scale in the exponent; their sum without it
-        const float shift = sc[1] - ref, inv = sc[2];
+        const float top = c == 0 ? top0 : top1;
+        float whole = sc[1];
+        if (top > -INFINITY) whole = fmaxf(whole, ref - kFar - floorf(top));
+        whole += kUpP - ref;
+        const float shift = whole + sc[2], inv = sc[3] * ex2(-whole - (m == -INFINITY ? 0.0f : m));
         const uint64_t f2 = pair(f, f), shift2 = pair(shift, shift), minus = pair(-1.0f, -1.0f);
         uint64_t sum = 0;
         auto put = [&](int e, uint64_t w) {
@@ -1156,7 +1160,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       if (tid == 0)  // one's own copies that may still be under way
         for (int k = max(0, nt - 2); k < nt; k++) tc::mbar_wait(code_full + 8 * (k & 1), (k >> 1) & 1, p.wait_limit);
     }
-    tops[0][half][local] = l;
+    tops[0][half][local] = l, tops[1][half][local] = m;
   }
   if (warp == 8 && lane == 0) {  // ---- products
     const uint32_t id_s = tc::make_idesc(0, kTile, kTile), id_o = tc::make_idesc(0, kTile, HDP);
@@ -1197,10 +1201,14 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   if (warp < 8) {
     const uint32_t mine = (uint32_t)(quad * 32) << 16;
     const bool sees = row < nrows && sight.limit(row / p.G) > 0;
-    const float total = tops[0][0][local] + tops[0][1][local];
-    const float unit_of = 1.0f / (1 << kUpP), inv = pp.splits == 1 ? unit_of / total : unit_of;
+    const float m0 = tops[1][0][local], m1 = tops[1][1][local], M = fmaxf(m0, m1);
+    const float total = tops[0][0][local] * rescale(m0, M) + tops[0][1][local] * rescale(m1, M);
     if (pp.splits > 1 && row < nrows && half == 0)
-      *(float2 *)(p.pml + (((size_t)unit * pp.splits + split) * nrows + row) * 2) = make_float2(m, total);
+      *(float2 *)(p.pml + (((size_t)unit * pp.splits + split) * nrows + row) * 2) = make_float2(M, total);
+    // from the references of the sums to the weights': 2^(end - M), in two steps, which an f32 has room for
+    const float end = fmaxf(run_ref, tile_ref), tile = rescale(tile_ref, end), old = rescale(run_ref, end), away = fminf(fmaxf(end - M, -250.0f), 250.0f);
+    const float part1 = floorf(away * 0.5f), part2 = ex2(away - part1);
+    const float inv = (pp.splits == 1 ? 1.0f / total : 1.0f) * (1.0f / (1 << kUpP)), up = ex2(part1);
 #pragma unroll 1
     for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
       uint32_t v[16];
@@ -1211,11 +1219,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         tc::tmem_ld_wait();
         if (nt > 1) {
 #pragma unroll
-          for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(y[e]) + __uint_as_float(v[e]));
+          for (int e = 0; e < 16; e++) v[e] = __float_as_uint(fmaf(__uint_as_float(y[e]), old, __uint_as_float(v[e]) * tile));
         }
       }
 #pragma unroll
-      for (int e = 0; e < 16; e++) v[e] = nt > 0 && sees ? __float_as_uint(__uint_as_float(v[e]) * inv * svmax) : 0u;
+      for (int e = 0; e < 16; e++) v[e] = nt > 0 && sees ? __float_as_uint(__uint_as_float(v[e]) * inv * up * part2) : 0u;
 #pragma unroll
       for (int e = 0; e < 16; e += 4) *(uint4 *)(so + local * PITCH + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
