@@ -375,6 +375,11 @@ def step_streams(ctx, dec, kv, st, x, n: int):
     return _step(ctx, dec, kv, st, x, n, st["S"])
 
 
+def _need_rules(ctx, rules) -> None:
+    if rules is not None and not hasattr(ctx, "pickAdjusted"):
+        raise ValueError("rules need a backend with pickAdjusted: a pick on the host would leave them out")
+
+
 def _pick(ctx, st, logits, VOCAB, rules):
     """The next token of each stream on the device: [S, 2] = {index, value}.  Under `rules` the picks so far (st["hist"],
     [rows, S], its first st["picked"] rows) are the history, and the pick joins it."""
@@ -413,6 +418,7 @@ def prefill_streams(ctx, dec, kv, st, tokens, want_logits: bool = False, rules: 
         raise ValueError("prefill_streams: a token id below 0 (a stream whose rules allowed no token)")
     if rules is not None and want_logits:
         raise ValueError("prefill_streams: rules are for the pick on the device")
+    _need_rules(ctx, rules)
     if n + T > dec["pos"].shape[0]:  # (a slice that ends early would be broadcast over the tokens)
         raise IndexError(f"prefill_streams: positions {n}..{n + T - 1} of a table of {dec['pos'].shape[0]}")
     emb = dec["embed"][tokens] + dec["pos"][n:n + T][None, :, :]
@@ -445,6 +451,7 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
     Returns int64 [S, n_tokens].  cache="int8": caches made here are 8-bit ones, and a state with such caches takes the prefix
     in one step; `lens` as in cross_kv_streams, `rules` as in decode_next_streams (the history: the tokens picked here)."""
     S = len(encs)
+    _need_rules(ctx, rules)
     own_kv, own_st = kv is None, st is None
     kv = cross_kv_streams(ctx, dec, encs, cache, lens=lens) if own_kv else kv
     try:

@@ -30,3 +30,17 @@ def test_tokens_behind_the_position_table(setup):
     for n, T in ((table - 1, 2), (table - 1, 5), (table, 2), (0, table + 1)):
         with pytest.raises(IndexError):
             wd.prefill_streams(ctx, dec, kv, dict(n=n, S=S, self8=[]), np.ones((S, T)))
+
+
+def test_rules_are_refused_where_nobody_follows_them(setup):
+    """The oracle has no pickAdjusted: its pick on the host would be the plain one."""
+    wd, ctx, dec, encs, S = setup
+    assert not hasattr(ctx, "pickAdjusted")
+    kv, st = wd.cross_kv_streams(ctx, dec, encs), wd.decode_init_streams(ctx, dec, S, 8)
+    for rules in (dict(presence=1e6), dict()):
+        for call in (lambda: wd.decode_next_streams(ctx, dec, kv, st, [1] * S, rules=rules), lambda: wd.prefill_streams(ctx, dec, kv, st, np.ones((S, 1)), rules=rules),
+                     lambda: wd.greedy_decode_streams(ctx, dec, encs, [1, 2], 3, rules=rules)):
+            with pytest.raises(ValueError, match="pickAdjusted"):
+                call()
+    assert st["n"] == 0
+    wd.greedy_decode_streams(ctx, dec, encs, [1, 2], 3)
