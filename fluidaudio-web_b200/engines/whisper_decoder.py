@@ -380,16 +380,18 @@ def _need_rules(ctx, rules) -> None:
         raise ValueError("rules need a backend with pickAdjusted: a pick on the host would leave them out")
 
 
-def _pick(ctx, st, logits, VOCAB, rules):
-    """The next token of each stream on the device: [S, 2] = {index, value}.  Under `rules` the picks so far (st["hist"],
-    [rows, S], its first st["picked"] rows) are the history, and the pick joins it."""
+def _pick(ctx, st, logits, VOCAB, rules, n):
+    """The next token of each stream on the device: [S, 2] = {index, value}, after a step from position n to st["n"].  Under
+    `rules` the picks so far (st["hist"], [rows, S]; st["picked"]: the positions that they were made for) are the history, and the
+    pick joins it.  Picks for positions behind n are of a run that the state was set back from: they are dropped."""
     if rules is None:
         return ctx.argmaxRowsIndex(logits, VOCAB)
     if "hist" not in st:
-        st["hist"], st["picked"] = ctx.pin(ctx.alloc(st["maxLen"], st["S"])), 0
-    pick = ctx.pickAdjusted(logits, VOCAB, history=st["hist"], n=st["picked"], **rules)
-    ctx.copyRows(st["hist"], ctx.reshapeView(ctx.sliceCols(pick, 0, 1), 1, st["S"]), st["picked"])
-    st["picked"] += 1
+        st["hist"], st["picked"] = ctx.pin(ctx.alloc(st["maxLen"], st["S"])), []
+    st["picked"] = [p for p in st["picked"] if p <= n]
+    pick = ctx.pickAdjusted(logits, VOCAB, history=st["hist"], n=len(st["picked"]), **rules)
+    ctx.copyRows(st["hist"], ctx.reshapeView(ctx.sliceCols(pick, 0, 1), 1, st["S"]), len(st["picked"]))
+    st["picked"].append(st["n"])
     return pick
 
 
@@ -397,7 +399,8 @@ def decode_next_streams(ctx, dec, kv, st, tokens: Sequence[int], want_logits: bo
     """One token per stream.  Returns (next token ids [S] by first-maximum argmax over the VOCAB real
     columns, logits [S, VOCAB] or None).  The token pick runs on the device when the backend has
     argmaxRowsIndex (8 bytes per stream come back instead of a logits row), else on the host.  With `rules` the pick is
-    pickAdjusted's (its history: the tokens that calls with rules have picked on this state so far); a stream that may pick
+    pickAdjusted's (its history: the tokens that calls with rules have picked on this state so far, up to the position that st["n"] was set back
+    to, if it was); a stream that may pick
     nothing gets -1."""
     return prefill_streams(ctx, dec, kv, st, np.asarray(tokens, dtype=np.int64).reshape(-1, 1), want_logits, rules)
 
@@ -430,7 +433,7 @@ def prefill_streams(ctx, dec, kv, st, tokens, want_logits: bool = False, rules: 
         logits = step_streams(ctx, dec, kv, st, x, n)
         st["n"] = n + T
         if on_device:
-            return ctx.stageDownload(_pick(ctx, st, logits, VOCAB, rules))
+            return ctx.stageDownload(_pick(ctx, st, logits, VOCAB, rules, n))
         return ctx.stageDownload(logits)
 
     try:
@@ -456,7 +459,7 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
     kv = cross_kv_streams(ctx, dec, encs, cache, lens=lens) if own_kv else kv
     try:
         st = decode_init_streams(ctx, dec, S, len(prefix) + n_tokens, cache) if own_st else st
-        st["n"] = st["picked"] = 0
+        st["n"], st["picked"] = 0, []
         nxt = None
         if "self8" in st:
             nxt, _ = prefill_streams(ctx, dec, kv, st, np.tile(np.asarray(prefix, np.int64), (S, 1)), rules=rules)

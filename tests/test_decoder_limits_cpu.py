@@ -5,6 +5,26 @@ import pytest
 from oracle.wasm_oracle import WasmOracle
 
 
+class WithRules(WasmOracle):
+    """The oracle with the members of the pick on the device, on the host: a presence penalty, a mask [VOCAB] or [S, VOCAB] of truth values."""
+
+    def argmaxRowsIndex(self, x, ncols=0):
+        return self.pickAdjusted(x, ncols)
+
+    def pickAdjusted(self, x, ncols=0, *, history=None, n=0, presence=0.0, mask=None):
+        y = x.array()[:, :ncols].copy()
+        assert history is None or n <= history.rows
+        for row in history.array()[:n] if n else ():
+            for s, t in enumerate(row):
+                if t >= 0:
+                    y[s, int(t)] -= presence
+        if mask is not None:
+            y = np.where(mask, y, -np.inf)
+        best = y.argmax(1)
+        value = y.max(1)
+        return self.upload(np.stack([np.where(value > -np.inf, best, -1), value], 1).astype(np.float32), x.rows, 2)
+
+
 @pytest.fixture
 def setup(pkg):
     from fluidaudio_web_b200.engines import synth, whisper_decoder as wd
@@ -44,3 +64,26 @@ def test_rules_are_refused_where_nobody_follows_them(setup):
                 call()
     assert st["n"] == 0
     wd.greedy_decode_streams(ctx, dec, encs, [1, 2], 3)
+
+
+def test_history_of_a_state_that_is_set_back(setup):
+    """Picks behind the position that a state is set back to are of another run; those in front of it stay."""
+    wd, _, dec, encs, S = setup
+    ctx = WithRules()
+    kv, st = wd.cross_kv_streams(ctx, dec, encs), wd.decode_init_streams(ctx, dec, S, 6)
+    rules = dict(presence=1e6)
+
+    def run(state, first, count):
+        out, t = [], first
+        for _ in range(count):
+            t = wd.decode_next_streams(ctx, dec, kv, state, t, rules=rules)[0]
+            out.append(t.tolist())
+        return out
+
+    want = run(wd.decode_init_streams(ctx, dec, S, 6), [1] * S, 6)
+    assert all(len({r[s] for r in want}) == 6 for s in range(S))
+    for _ in range(3):
+        st["n"] = 0
+        assert run(st, [1] * S, 6) == want
+    st["n"] = 2  # the two tokens before it count, the four behind it do not
+    assert run(st, want[1], 4) == want[2:]
