@@ -399,9 +399,8 @@ def decode_next_streams(ctx, dec, kv, st, tokens: Sequence[int], want_logits: bo
     """One token per stream.  Returns (next token ids [S] by first-maximum argmax over the VOCAB real
     columns, logits [S, VOCAB] or None).  The token pick runs on the device when the backend has
     argmaxRowsIndex (8 bytes per stream come back instead of a logits row), else on the host.  With `rules` the pick is
-    pickAdjusted's (its history: the tokens that calls with rules have picked on this state so far, up to the position that st["n"] was set back
-    to, if it was); a stream that may pick
-    nothing gets -1."""
+    pickAdjusted's (its history: the tokens that calls with rules have picked on this state so far, up to the position that
+    st["n"] was set back to, if it was); a stream that may pick nothing gets -1."""
     return prefill_streams(ctx, dec, kv, st, np.asarray(tokens, dtype=np.int64).reshape(-1, 1), want_logits, rules)
 
 
@@ -452,7 +451,8 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
                           kv=None, st=None, cache: Optional[str] = None, lens=None, rules: Optional[dict] = None) -> np.ndarray:
     """S clips decoded in lock step: the forced prefix, then n_tokens greedy tokens per stream.
     Returns int64 [S, n_tokens].  cache="int8": caches made here are 8-bit ones, and a state with such caches takes the prefix
-    in one step; `lens` as in cross_kv_streams, `rules` as in decode_next_streams (the history: the tokens picked here)."""
+    in one step; `lens` as in cross_kv_streams, `rules` as in decode_next_streams (the history: the tokens picked here).  A
+    stream that may pick nothing has ended: its tokens are -1 from there on, the others go on."""
     S = len(encs)
     _need_rules(ctx, rules)
     own_kv, own_st = kv is None, st is None
@@ -466,11 +466,15 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
         else:
             for i, t in enumerate(prefix):
                 nxt, _ = decode_next_streams(ctx, dec, kv, st, [int(t)] * S, rules=rules if i + 1 == len(prefix) else None)
-        out = np.empty((S, n_tokens), np.int64)
+        out = np.full((S, n_tokens), -1, np.int64)
+        ended = np.zeros(S, bool)
         for i in range(n_tokens):
-            out[:, i] = nxt
-            if i + 1 < n_tokens:
-                nxt, _ = decode_next_streams(ctx, dec, kv, st, nxt, rules=rules)
+            ended |= np.asarray(nxt) < 0
+            if ended.all():
+                break
+            out[:, i] = np.where(ended, -1, nxt)
+            if i + 1 < n_tokens:  # (an ended stream is fed token 0: nobody sees what it would say)
+                nxt, _ = decode_next_streams(ctx, dec, kv, st, np.where(ended, 0, nxt), rules=rules)
         return out
     finally:
         free_caches(ctx, kv if own_kv else None, st if own_st else None)

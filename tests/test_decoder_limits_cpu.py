@@ -9,7 +9,7 @@ class WithRules(WasmOracle):
     """The oracle with the members of the pick on the device, on the host: a presence penalty, a mask [VOCAB] or [S, VOCAB] of truth values."""
 
     def argmaxRowsIndex(self, x, ncols=0):
-        return self.pickAdjusted(x, ncols)
+        return WithRules.pickAdjusted(self, x, ncols)
 
     def pickAdjusted(self, x, ncols=0, *, history=None, n=0, presence=0.0, mask=None):
         y = x.array()[:, :ncols].copy()
@@ -87,3 +87,35 @@ def test_history_of_a_state_that_is_set_back(setup):
         assert run(st, [1] * S, 6) == want
     st["n"] = 2  # the two tokens before it count, the four behind it do not
     assert run(st, want[1], 4) == want[2:]
+
+
+@pytest.mark.parametrize("n", [1, 7])
+def test_a_stream_that_may_pick_nothing_ends_alone(setup, n):
+    """A few tokens are allowed for stream 0, each once: it ends behind the last of them.  The other stream decodes as it does without it."""
+    wd, _, dec, encs, S = setup
+    ctx = WithRules()
+    V = dec["cfg"]["VOCAB"]
+
+    class Taking(WithRules):
+        def __init__(self, only):
+            super().__init__()
+            self.left = np.ones((S, V), bool)
+            self.left[0] = np.isin(np.arange(V), only)
+
+        def pickAdjusted(self, x, ncols=0, **kw):
+            pick = super().pickAdjusted(x, ncols, mask=self.left, **kw)
+            t = int(pick.array()[0, 0])
+            if t >= 0:
+                self.left[0, t] = False
+            return pick
+
+    got = {}
+    for only in ([3, 50, 7, 120, 9], [3], []):
+        out = wd.greedy_decode_streams(Taking(only), dec, encs, [1, 2], n, rules=dict(presence=1e6))
+        have = min(n, len(only))
+        assert set(out[0, :have]) <= set(only) and len(set(out[0, :have])) == have and (out[0, have:] == -1).all()
+        got[len(only)] = out[1].tolist()
+    want = wd.greedy_decode_streams(ctx, dec, encs, [1, 2], n, rules=dict(presence=1e6))[1].tolist()
+    assert all(r == want for r in got.values()) and min(want) >= 0
+    none = dict(mask=np.zeros(V, bool))
+    assert (wd.greedy_decode_streams(ctx, dec, encs, [1, 2], n, rules=none) == -1).all()
