@@ -327,29 +327,37 @@ def cross_kv_streams(ctx, dec, encs, cache: Optional[str] = None, S: int = 0, le
     if lens is not None and not cache:
         raise ValueError("cross_kv_streams: lengths of the clips' own need 8-bit caches")
     cfg = dec["cfg"]
-    for w in dec["layers"]:
-        k = ctx.pin(_mm(ctx, enc_all, w["ckw"]))
-        v = ctx.pin(_mm(ctx, enc_all, w["cvw"], bias=w["cvb"]))
-        if cache:
-            n = enc_all.rows // S
-            try:
+    own = []  # tensors that do not outlive this call
+    try:
+        for w in dec["layers"]:
+            own.append(ctx.pin(_mm(ctx, enc_all, w["ckw"])))
+            own.append(ctx.pin(_mm(ctx, enc_all, w["cvw"], bias=w["cvb"])))
+            k, v = own
+            if cache:
+                n = enc_all.rows // S
                 out.append(dict(cache=ctx.kvCache8(S, n, cfg["NH"], cfg["HD"]), n=n, lens=lens))
                 ctx.kvWrite8(out[-1]["cache"], k, v, counts=lens)
-            except Exception:
-                free_caches(ctx, out)
-                raise
-            finally:
-                ctx.freeTensor(k)
-                ctx.freeTensor(v)
-        else:
-            out.append(dict(k=k, v=v))
+                for t in own:
+                    ctx.freeTensor(t)
+            else:
+                out.append(dict(k=k, v=v))
+            own = []
+    except Exception:
+        free_caches(ctx, out)
+        for t in own + [e[m] for e in out if not cache for m in "kv"]:
+            ctx.freeTensor(t)
+        raise
     return out
 
 
 def free_caches(ctx, kv: Optional[list] = None, st: Optional[dict] = None) -> None:
-    """Gives the 8-bit caches of cross_kv_streams and decode_init_streams back."""
-    for c in [e["cache"] for e in kv or [] if "cache" in e] + (st or {}).get("self8", []):
+    """Gives the 8-bit caches of cross_kv_streams and decode_init_streams back, and a state's history of picks under rules."""
+    st = st or {}
+    for c in [e["cache"] for e in kv or [] if "cache" in e] + st.get("self8", []):
         ctx.freeKvCache8(c)
+    if "hist" in st:
+        ctx.freeTensor(st.pop("hist"))
+        st.pop("picked")
 
 
 def decode_init_streams(ctx, dec, S: int, maxLen: int = 448, cache: Optional[str] = None) -> dict:
@@ -478,8 +486,6 @@ def greedy_decode_streams(ctx, dec, encs: Sequence, prefix: Sequence[int], n_tok
         return out
     finally:
         free_caches(ctx, kv if own_kv else None, st if own_st else None)
-        if own_st and st and "hist" in st:
-            ctx.freeTensor(st["hist"])
 
 
 # ---------------------------------------------------------------------------- device-resident greedy loop

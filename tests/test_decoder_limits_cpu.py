@@ -119,3 +119,67 @@ def test_a_stream_that_may_pick_nothing_ends_alone(setup, n):
     assert all(r == want for r in got.values()) and min(want) >= 0
     none = dict(mask=np.zeros(V, bool))
     assert (wd.greedy_decode_streams(ctx, dec, encs, [1, 2], n, rules=none) == -1).all()
+
+
+class Counting(WithRules):
+    """Which tensors are pinned and not given back; 8-bit caches that hold nothing; the `fail`-th product fails."""
+
+    def __init__(self, fail=0):
+        super().__init__()
+        self.live, self.products, self.fail = {}, 0, fail
+
+    def matmul(self, *a, **kw):
+        self.products += 1
+        if self.products == self.fail:
+            raise MemoryError("no room")
+        return super().matmul(*a, **kw)
+
+    def pin(self, t, toParent=False):
+        self.live[id(t)] = t
+        return t
+
+    def freeTensor(self, t):
+        self.live.pop(id(t), None)
+
+    def kvCache8(self, *shape):
+        return self.pin(object())
+
+    def kvWrite8(self, cache, *a, **kw):
+        pass
+
+    def freeKvCache8(self, cache):
+        self.freeTensor(cache)
+
+
+@pytest.mark.parametrize("cache", [None, "int8"])
+def test_what_was_made_goes_back_when_a_product_fails(setup, cache):
+    wd, _, dec, encs, S = setup
+    products = 2 * len(dec["layers"])
+    for fail in range(1, products + 1):
+        ctx = Counting(fail)
+        with pytest.raises(MemoryError):
+            wd.cross_kv_streams(ctx, dec, encs, cache)
+        assert ctx.products == fail and not ctx.live
+    ctx = Counting()
+    kv = wd.cross_kv_streams(ctx, dec, encs, cache)
+    assert len(ctx.live) == (len(dec["layers"]) if cache else products)
+    wd.free_caches(ctx, kv)
+    assert len(ctx.live) == (0 if cache else products)
+
+
+def test_a_states_history_goes_back(setup):
+    wd, _, dec, encs, S = setup
+    ctx = Counting()
+    kv, st = wd.cross_kv_streams(ctx, dec, encs), wd.decode_init_streams(ctx, dec, S, 6)
+    before = set(ctx.live)
+    first = wd.decode_next_streams(ctx, dec, kv, st, [1] * S, rules=dict(presence=1e6))[0].tolist()
+    assert len(ctx.live) == len(before) + 1
+    wd.free_caches(ctx, kv, st)
+    assert set(ctx.live) == before
+    wd.free_caches(ctx, kv, st)  # twice is no error
+    st["n"] = 0
+    assert wd.decode_next_streams(ctx, dec, kv, st, [1] * S, rules=dict(presence=1e6))[0].tolist() == first
+    # a history that the loop made for a state of its own, and one that stays with the caller's
+    held = len(ctx.live)
+    wd.greedy_decode_streams(ctx, dec, encs, [1, 2], 3, kv=kv, st=st, rules=dict(presence=1e6))
+    assert len(ctx.live) == held
