@@ -113,6 +113,10 @@ extern "C" int fa_decoder_step_kv8(fa_ctx *ctx, const fa_decoder_layer *layers, 
   FA_REQUIRE(ctx, fa_valid(ctx, x) && n_layers > 0 && fa_valid_kv8(ctx, self[0]), "decoderStepKv8: unknown handle");
   const int S = self[0]->S, T = x->rows / S, D = x->cols;
   FA_REQUIRE(ctx, T >= 1 && x->rows % S == 0, "decoderStepKv8: %d rows for %d streams", x->rows, S);
+  for (int l = 0; l < n_layers; l++) {  // (rows that fit another number of streams would meet other streams' keys)
+    FA_REQUIRE(ctx, fa_valid_kv8(ctx, cross[l]) && fa_valid_kv8(ctx, self[l]), "decoderStepKv8: unknown cache handle, layer %d", l);
+    FA_REQUIRE(ctx, self[l]->S == S && S % cross[l]->S == 0, "decoderStepKv8: layer %d: caches of %d and %d streams for %d", l, cross[l]->S, self[l]->S, S);
+  }
   ArenaScope scope(ctx);
   FA_TRY(scope.open());
   fa_tensor *cur = nullptr, *y = nullptr;

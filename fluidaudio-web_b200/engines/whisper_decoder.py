@@ -216,6 +216,9 @@ def _layer_kv8(ctx, x, w, kv, cache, n, NH):
 
 def _step_kv8(ctx, dec, kv, st, x, n, S, native):
     cfg = dec["cfg"]
+    for clips, own in zip([e["cache"].S for e in kv], [c.S for c in st["self8"]]):
+        if own != S or S % clips:  # (rows that fit would meet other streams' keys)
+            raise ValueError(f"8-bit caches of {clips} clips and {own} streams for {S} streams")
     if None not in native and hasattr(ctx, "decoderStepKv8"):
         return ctx.decoderStepKv8(native, x, [c["cache"] for c in kv], kv[0]["n"], st["self8"], n, cfg["NH"], dec["lnf"], dec["embedT"].native(),
                                   lens=kv[0]["lens"])

@@ -317,7 +317,7 @@ int fa_decoder_step(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, c
                     const fa_tensor *lnf_w, const fa_tensor *lnf_b, const fa_linear *logits, fa_tensor **out);
 /* The same over 8-bit caches, for T >= 1 tokens of each of S streams (a prompt, or one token): x [S*T, D], stream-major, tokens
  * at positions n .. n+T-1 -> logits of each stream's last token [S, N].  cross, self: one cache per layer; the cross caches
- * hold n_cross positions, or lens[s] of them (fa_attn_kv8). */
+ * hold n_cross positions, or lens[s] of them (fa_attn_kv8), of S streams or of S/b: b neighbouring streams then share a clip. */
 int fa_decoder_step_kv8(fa_ctx *ctx, const fa_decoder_layer *layers, int n_layers, const fa_tensor *x, fa_kv8 *const *cross,
                         const fa_tensor *lens, int n_cross, fa_kv8 *const *self, int n, int NH, const fa_tensor *lnf_w,
                         const fa_tensor *lnf_b, const fa_linear *logits, fa_tensor **out);
