@@ -420,6 +420,9 @@ __host__ __device__ constexpr size_t smem_bytes(int rows = Acc::ROWS) {
 // What a unit costs a warp beside its blocks (queries, its result), in blocks: shares of the list are equal with it.
 constexpr int kTurn = 4;
 constexpr int kLeast = 2;  // places of a warp's share at least
+// Places of a launch at most, unless one group of rows alone has more: the kernel counts them in 32 bits, a warp's share beyond the
+// end included.  Several launches of 2^24 places take milliseconds each, so that what a further one costs does not show.
+constexpr long long kMostPlaces = 1 << 24;
 
 // Result row from its parts: maximum and sum of weights, channels lane, lane + 32, ...
 template <int HDP>
@@ -742,11 +745,11 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
   static SmemLimit limit;
   FA_CHECK_CUDA(ctx, limit.raise(ctx, k_attn_kv8<HDP, Acc>, smem_bytes<HDP, Acc>()));
   const int nb = ceil_div(most < 1 ? 1 : most, kBlock), groups = ceil_div(p.G * p.T, ROWS);
-  const long long list = (long long)c->S * c->H * (nb + kTurn);  // places of a row group, < 2^31: the cache fits the device
+  const long long list = (long long)c->S * c->H * (nb + kTurn);  // places of a row group, < 2^29: the cache fits the device
   const int rows = p.G * p.T < ROWS ? p.G * p.T : ROWS, slots = ctx->sm_count * resident<HDP, Acc>(rows);
   int rc = FA_OK;
   for (p.rg0 = 0; p.rg0 < groups && rc == FA_OK; p.rg0 += p.rowgroups) {
-    const long long fit = 0x7fffffffLL / list;
+    const long long fit = list < kMostPlaces ? kMostPlaces / list : 1;
     p.rowgroups = (int)(groups - p.rg0 < fit ? groups - p.rg0 : fit);
     const long long share = (list * p.rowgroups + kWarps * kLeast - 1) / (kWarps * kLeast);
     const int grid = (int)(share < slots ? share : slots);
