@@ -213,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_adjust(const Logi
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
-    p.out[2 * s] = at == 0x7fffffff ? -1.0f : (float)at;
-    p.out[2 * s + 1] = best;
+    p.out[2 * (long long)s] = at == 0x7fffffff ? -1.0f : (float)at;
+    p.out[2 * (long long)s + 1] = best;
   }
   if (nc > 1) cluster_sync();  // no block leaves while its result is read
 }
