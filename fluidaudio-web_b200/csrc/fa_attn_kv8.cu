@@ -753,7 +753,8 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
     p.rowgroups = (int)(groups - p.rg0 < fit ? groups - p.rg0 : fit);
     const long long share = (list * p.rowgroups + kWarps * kLeast - 1) / (kWarps * kLeast);
     const int grid = (int)(share < slots ? share : slots);
-    const size_t part = (size_t)grid * 2 * rows, tickets = p.rowgroups > 1 ? (size_t)c->S * c->H * p.rowgroups : 0;
+    // room for all thread blocks that the GPU holds, whatever the grid: a cache that grows block by block wants the same memory
+    const size_t part = (size_t)slots * 2 * rows, tickets = p.rowgroups > 1 ? (size_t)c->S * c->H * p.rowgroups : 0;
     void *scratch = nullptr;
     size_t bytes = 0;
     FA_TRY(fa_block_acquire(ctx, part * (HDP + 2) * 4 + tickets * 4, &scratch, &bytes));
