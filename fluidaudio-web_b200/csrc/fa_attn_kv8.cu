@@ -800,7 +800,8 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 // positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.
 constexpr int kPromptRows = 49;
 constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6;
-// A block's products are at least 2^-kFar of the row's largest ones (as f16 that is 0 all the same): its sum of weights needs them.
+// A block's scale is taken for so large at least that a weight at the row's maximum gives 2^-kFar of the largest product (0, as
+// f16): products as small as f32 may have them would take the weights out of their sum.
 constexpr float kFar = 80.0f;
 
 template <int HDP>
@@ -1023,7 +1024,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         const float f = sc.y < INFINITY ? __uint_as_float((bits & 0x7fffffu) | 0x3f800000u) : __int_as_float(0x7fc00000);
         scl[k & 1][quad][0] = sc.x * kScoreUnit;
         scl[k & 1][quad][1] = sc.y > 0.0f ? (float)((int)(bits >> 23) - (small ? 191 : 127)) : -200.0f;
-        scl[k & 1][quad][2] = log2f(f), scl[k & 1][quad][3] = 1.0f / f;
+        const float lf = __log2f(f);
+        scl[k & 1][quad][2] = lf, scl[k & 1][quad][3] = ex2(-lf);
       }
       tc::fence_proxy_async_smem();
       arrive(k_full);
@@ -1081,7 +1083,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
       __syncwarp();
       tc::tc_fence_after();
       const int seen = lim - (t0 + k) * kTile - 64 * half;  // of this thread's 64 positions
-      float top0 = -INFINITY, top1 = -INFINITY;  // of the two blocks
+      float top = -INFINITY, most_of = -INFINITY;  // the largest score, the largest product of a weight and a scale
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         float v[32];
@@ -1095,20 +1097,19 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
 #pragma unroll
           for (int e = 0; e < 32; e++) t = e < n ? fmaxf(t, v[e]) : t;
         }
-        t = n > 0 ? fmaxf(-INFINITY, t * (scl[k & 1][2 * half + c][0] * qs)) : -INFINITY;  // (NaN: no maximum)
-        if (c == 0) top0 = t;
-        else top1 = t;
+        const float *sc = scl[k & 1][2 * half + c];
+        if (n > 0) t *= sc[0] * qs, top = fmaxf(top, t), most_of = fmaxf(most_of, t + sc[1]);  // (a NaN is no maximum)
       }
-      // the row's largest product of a weight and a scale, the other half's too
-      float most_of = fmaxf(top0 + scl[k & 1][2 * half][1], top1 + scl[k & 1][2 * half + 1][1]);
+      // the product's largest for the whole row: the other half's too
       tops[k & 1][half][local] = most_of;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
       most_of = floorf(fmaxf(most_of, tops[k & 1][1 - half][local]));
       if (k > 0) sum_up(k > 1);
       tile_ref = most_of;
-      const float ref = tile_ref == -INFINITY ? 0.0f : tile_ref, next = fmaxf(m, floorf(fmaxf(top0, top1)));
+      const float ref = tile_ref == -INFINITY ? 0.0f : tile_ref, next = fmaxf(m, floorf(top));
       l *= rescale(m, next);
       m = next;
+      const float m_or_0 = m == -INFINITY ? 0.0f : m, least_of = ref - kFar - m_or_0;
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         float v[32];
@@ -1119,11 +1120,8 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
         const float *sc = scl[k & 1][2 * half + c];
         const float f = sc[0] * qs;
         // weights with the values' scale in the exponent; their sum without it
-        const float top = c == 0 ? top0 : top1;
-        float whole = sc[1];
-        if (top > -INFINITY) whole = fmaxf(whole, ref - kFar - floorf(top));
-        whole += kUpP - ref;
-        const float shift = whole + sc[2], inv = sc[3] * ex2(-whole - (m == -INFINITY ? 0.0f : m));
+        const float whole = fmaxf(sc[1], least_of) + (kUpP - ref);
+        const float shift = whole + sc[2], inv = sc[3] * ex2(-whole - m_or_0);
         const uint64_t f2 = pair(f, f), shift2 = pair(shift, shift), minus = pair(-1.0f, -1.0f);
         uint64_t sum = 0;
         auto put = [&](int e, uint64_t w) {
