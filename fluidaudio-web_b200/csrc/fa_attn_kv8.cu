@@ -863,13 +863,14 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
   const AttnParams &p = pp.a;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
-  __shared__ __align__(8) uint64_t bar[8];  // see the names below
+  __shared__ __align__(8) uint64_t bar[9];  // see the names below
   __shared__ float tops[2][2][kTile];        // row maxima of the two halves; their sums of weights and maxima in the end
   __shared__ float scl[2][4][4];            // a tile's scales: keys, in units of log 2; values as 2^[1] * 2^[2], and 2^-[2]
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up;
   const uint32_t s_full = smem_u32(&bar[0]), p_full = smem_u32(&bar[1]), pv_done = smem_u32(&bar[2]), k_full = smem_u32(&bar[3]),
-                 v_full = smem_u32(&bar[4]), code_free = smem_u32(&bar[5]), code_full = smem_u32(&bar[6]);  // (two stages)
+                 v_full = smem_u32(&bar[4]), code_free = smem_u32(&bar[5]), code_full = smem_u32(&bar[6]),  // (two stages)
+                 drained = smem_u32(&bar[8]);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   int at = blockIdx.x;
@@ -885,6 +886,7 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
     tc::mbar_init(code_free, 8);
     tc::mbar_init(code_full, 1);
     tc::mbar_init(code_full + 8, 1);
+    tc::mbar_init(drained, 1);
     tc::fence_barrier_init();
     gave_up = 0;
   }
@@ -1192,7 +1194,11 @@ __global__ void __launch_bounds__(kPromptThreads, HDP <= 64 ? 2 : 1) k_prompt_kv
                   part + step > 0);
       tc::umma_commit(pv_done);
     }
-    if (!ok) gave_up = 1;
+    if (!ok) {  // products may still be under way: they read shared memory and write columns that are given back
+      gave_up = 1;
+      tc::umma_commit(drained);
+      tc::mbar_wait(drained, 0, p.wait_limit);
+    }
   }
   tc::tc_fence_before();
   __syncthreads();
