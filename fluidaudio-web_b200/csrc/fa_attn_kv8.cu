@@ -791,13 +791,14 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 // relative to the largest score; it takes the scales out of the sums of products again, a factor for each block.  References are whole
 // powers of two: what moves between them is not rounded.
 //
-// What bounds it: the softmax warps (about 6 instructions an element and one exponential, 16 a clock and SM) and the products,
-// 2 x 128 x 128 x HD x 2 x 2 a tile, cost about the same; two thread blocks an SM overlap them where shared memory allows.
-// A tile costs a thread block about 5900 cycles at two an SM, its start and end 20000.  8 streams of 224 queries, 20 heads of 64
-// over up to 1500 positions of different lengths: 56 us; 16 streams' prompts of 224 over themselves: write and attention 61 us.
+// What bounds it: the chain of a tile's scores, softmax and products, which two thread blocks an SM overlap where shared memory
+// allows, and a thread block's start and end, a few tiles' worth.  8 streams of 224 queries, 20 heads of 64 over up to 1500
+// positions of different lengths: 57 us, in which 2.1 of 4 instructions a clock are issued (23 a score, all in all) and the tensor
+// pipe is busy for 22 %; 16 streams' prompts of 224 over themselves: write and attention 54 us.
 // Separate warps for the softmax and the conversion took 70 us in place of 55, runs of four to eight tiles 72 to 80.
 // From this many rows of a unit on.  Measured, us, groups of 16 rows / this kernel, 16 streams of 20 heads of 64 over 1500
-// positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.
+// positions: 32 rows 62 / 95, 48 rows 81 / 99, 64 rows 96 / 95; one stream: 24 rows 25 / 20, 64 rows 27 / 19.  The rule goes by
+// the former, whose loss is the larger one; other widths and lengths were not measured for it.
 constexpr int kPromptRows = 49;
 constexpr int kTile = 128, kPromptThreads = 288, kUpP = 6;
 // A block's scale is taken for so large at least that a weight at the row's maximum gives 2^-kFar of the largest product (0, as

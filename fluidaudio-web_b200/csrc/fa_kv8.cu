@@ -221,10 +221,10 @@ __device__ __forceinline__ void write_block(const WriteParams &p, const T *src, 
 
 // One (stream, head, keys or values) and a run of blocks.  The thread block of x == 0 takes the last block that the rows touch
 // too, behind its own: the first may need the tail that the last one replaces.
-// Bound by HBM, 4 bytes in, 1 out, where rows are many, and then close to what the SMs issue (a run of four blocks shares
-// what a thread block has to find out first); by the latency of a load and two barriers for one row.  24 clips of 1500
-// positions, 20 heads of 64: f32 114 us = 4.1 TB/s in and out, f16 130; of lengths from 0 to 1500 62 us (81 with blocks one by
-// one; then ten thread blocks an SM 79, sixteen 106).
+// Where rows are many, bound by its own instructions, 32 a value at 2.9 of 4 a clock (a run of four blocks shares what a thread
+// block has to find out first), above the floor of HBM, 4 bytes in, 1 out; by the latency of a load and two barriers for one row.
+// 24 clips of 1500 positions, 20 heads of 64: f32 112 us = 4.1 TB/s in and out, f16 130; of lengths from 0 to 1500 62 us (81 with
+// blocks one by one; then ten thread blocks an SM 79, sixteen 106).
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kThreads, HDP <= 64 ? 8 : HDP <= 128 ? 5 : 3) k_kv8_write(const WriteParams p) {
   __shared__ __align__(16) uint32_t sw[8 * HDP];
