@@ -116,9 +116,10 @@ __device__ __forceinline__ float ex2(float x) {
 // 2^(m - M) for M >= m, 1 where the two are the same infinity
 __device__ __forceinline__ float rescale(float m, float M) { return m == M ? 1.0f : ex2(m - M); }
 
-// Weights and query rows are scaled by 2^kUp before they are split (f16 ends at 2^16, and the less of a residue is subnormal the
-// better); the weights' is in their sum too.
-constexpr int kUp = 14;
+// Query rows are scaled by 2^kUp and weights by about 2^kUpW before they are split (f16 ends at 2^16, and the less of a residue is
+// subnormal the better).  What weights are relative to is their block's largest score less kUpW as an f32 has it: where scores
+// are so large that the difference is rounded, it is off by at most 8, and it is the reference of the block's sums as well.
+constexpr int kUp = 14, kUpW = 7;
 constexpr float kScoreUnit = kLog2e / (1 << kUp);  // scores in units of log 2
 
 // Channels 16k + 4t ..+3 of query row `row` for all k, scaled by the power of two that brings its largest element to
@@ -219,9 +220,9 @@ struct FewRows {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const float ref = top == -INFINITY ? 0.0f : top - kUp, M = fmaxf(m, top), old = rescale(m, M), c = rescale(top, M);
+    const float ref = top - kUpW, M = fmaxf(m, ref), old = rescale(m, M), c = rescale(ref, M), from = ref == -INFINITY ? 0.0f : ref;
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = ex2(v[j] - ref);
+    for (int j = 0; j < 4; j++) v[j] = ex2(v[j] - from);
     l = fmaf(l, old, ((v[0] + v[1]) + (v[2] + v[3])) * c);
     m = M;
     const float add = lim > first ? c * scales.y : 0.0f;  // (a block that a row sees nothing of may hold NaN)
@@ -343,13 +344,13 @@ struct ManyRows {
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float ref = top == -INFINITY ? 0.0f : top - kUp, M = fmaxf(m[r], top), c = rescale(top, M);
+      const float ref = top - kUpW, M = fmaxf(m[r], ref), c = rescale(ref, M), from = ref == -INFINITY ? 0.0f : ref;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          v[j][e] = ex2(v[j][e] - ref);
+          v[j][e] = ex2(v[j][e] - from);
           sum += v[j][e];
         }
       const float old = rescale(m[r], M);

@@ -115,3 +115,36 @@ def test_values_of_any_size(ctx, cache, T, power):  # noqa: F811
     assert (np.abs(got(ctx, ctx.attnKv8(put(ctx, q), c, 1, n)) - want) <= bound).all()
     zero, _, _ = held(ctx, cache, k, np.zeros_like(v))
     assert not got(ctx, ctx.attnKv8(put(ctx, q), zero, 1, n)).any()
+
+
+@pytest.mark.parametrize("T", [t for t in ROWS if t < 49])
+@pytest.mark.parametrize("size", [30.0, 1e4, 1e7, 3e9, 1e20])
+def test_scores_of_any_size(ctx, cache, T, size):  # noqa: F811
+    """Two positions of a row share the largest score, in blocks whose values lie 2^30 apart, all others are as far below zero.
+    Keys are +-1 in the first channel, the only one that queries have, so that equal scores are equal in every form, and scores are
+    off by nothing that weights could show."""
+    n, HD = 420, 64
+    rng = np.random.default_rng(T)
+    k, v = rng.uniform(-1, 1, (n, HD)).astype(f32), make(rng, 1, n, HD)
+    k[:, 0] = -1
+    k[[40, 333], 0] = 1
+    v[320:352] *= f32(2.0 ** 30)
+    q = np.zeros((T, HD), f32)
+    q[:, 0] = size * (1 + np.arange(T) / 7)
+    c, K, V = held(ctx, cache, k, v)
+    for order in (1, -1):  # the small values' block first, and last
+        if order < 0:
+            k, v = k[::-1].copy(), v[::-1].copy()
+            v *= f32(2.0 ** -20)
+            c, K, V = held(ctx, cache, k, v)
+        a, b = np.flatnonzero(k[:, 0] > 0)
+        assert K[0, a, 0] == K[0, b, 0] and (K[0][k[:, 0] < 0, 0] == -K[0, a, 0]).all()
+        V64 = V[0].astype(np.float64)
+        want = (V64[a] + V64[b]) / 2
+        B = [np.abs(V64[i // 32 * 32:i // 32 * 32 + 32]).max() for i in (a, b)]
+        rest = n * np.exp(-2 * size) * np.abs(V64).max()
+        out = got(ctx, ctx.attnKv8(put(ctx, q), c, 1, n))
+        assert (np.abs(out - want) <= (2.0 ** -20 + (n / 32 + 64) * EPS) * (B[0] + B[1]) / 2 + n * 2.0 ** -31 * max(B) + rest).all()
+        # b is not seen: the first alone
+        out = got(ctx, ctx.attnKv8(put(ctx, q), c, 1, n, lens=put(ctx, [[b]])))
+        assert (np.abs(out - V64[a]) <= (2.0 ** -20 + (n / 32 + 64) * EPS + n * 2.0 ** -31) * B[0] + rest).all()
