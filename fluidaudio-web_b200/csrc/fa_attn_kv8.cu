@@ -790,7 +790,9 @@ int run(fa_ctx *ctx, const fa_kv8 *c, AttnParams &p, int most, const char *label
 // What other rows see, or blocks that a row gives no weight to, however large their values, is not in it.  A tile's result
 // joins the running one, which has a reference of its own and lies in TMEM beside it.  The sum of the weights alone is kept
 // relative to the largest score; it takes the scales out of the sums of products again, a factor for each block.  References are whole
-// powers of two: what moves between them is not rounded.
+// powers of two: what moves between them is not rounded, up to scores of 2^23.  (Weights formed relative to their own block's largest
+// and multiplied with its scale afterwards would take scores of any size and no logarithm of a scale: 64 us in place of 57, the same
+// error.)
 //
 // What bounds it: the chain of a tile's scores, softmax and products, which two thread blocks an SM overlap where shared memory
 // allows, and a thread block's start and end, a few tiles' worth.  8 streams of 224 queries, 20 heads of 64 over up to 1500

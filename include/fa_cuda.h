@@ -293,7 +293,8 @@ int fa_kv8_read(fa_ctx *ctx, fa_kv8 *cache, int row0, int rows, fa_tensor **out_
 /* softmax(q K^T) V over positions 0..n-1, or 0..lens[s]-1 (lens[s] <= n), for T queries per stream: q [S*T, HQ*HD] ->
  * [S*T, HQ*HD].  HQ is a multiple of H: HQ / H neighbouring query heads share a key head.  A stream of length 0 gives zeros.
  * q carries 1/sqrt(HD) as for fa_attn_step.  f32-grade: operands in 22 bits, sums in f32, relative to what a query itself adds
- * up: values of other blocks that it does not see, or gives no weight to, take nothing from its result however large. */
+ * up: values of other blocks that it does not see, or gives no weight to, take nothing from its result however large.
+ * From 49 rows of a key head on (queries x query heads that share it), scores q k are expected below 2^23. */
 int fa_attn_kv8(fa_ctx *ctx, const fa_tensor *q, fa_kv8 *cache, int HQ, int n, const fa_tensor *lens, fa_tensor **out);
 /* The self-attention form: qkv [S*T, (HQ + 2H)*HD] holds q | k | v of T new tokens per stream; writes them as fa_kv8_write
  * does, then query i attends over positions 0 .. n + i (pos[s] + i) as they are stored now.  Rows i >= counts[s] give zeros. */
